@@ -214,4 +214,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   register_attention_sm100_ops(m);
   register_pscore_sm100_ops(m);
   register_token_prune_ops(m);
+  register_packed_layout_ops(m);
+  register_packed_rope_ops(m);
+  register_packed_attention_ops(m);
 }

@@ -14,4 +14,7 @@ void register_conv_ops(pybind11::module_& m);
 void register_attention_sm100_ops(pybind11::module_& m);
 void register_pscore_sm100_ops(pybind11::module_& m);
 void register_token_prune_ops(pybind11::module_& m);
+void register_packed_layout_ops(pybind11::module_& m);
+void register_packed_rope_ops(pybind11::module_& m);
+void register_packed_attention_ops(pybind11::module_& m);
 }  // namespace appcorr
