@@ -33,23 +33,6 @@ constexpr int kFaBN = 128;   // keys per block
 constexpr int kFaThreads = 192;
 constexpr float kRescaleThreshold = 8.0f;  // log2 units
 
-// Shared-memory descriptor for an MN-major operand tile with the 128-byte swizzle: 8 K-rows of
-// 128 B (64 MN elements) per atom, atoms along K `sbo` bytes apart, along MN `lbo` bytes apart.
-__device__ __forceinline__ uint64_t sw128_mnmajor_desc(uint32_t smem_byte_addr, uint32_t lbo, uint32_t sbo) {
-  uint64_t d = 0;
-  d |= static_cast<uint64_t>((smem_byte_addr >> 4) & 0x3FFF);
-  d |= static_cast<uint64_t>((lbo >> 4) & 0x3FFF) << 16;
-  d |= static_cast<uint64_t>((sbo >> 4) & 0x3FFF) << 32;
-  d |= static_cast<uint64_t>(1) << 46;
-  d |= static_cast<uint64_t>(2) << 61;
-  return d;
-}
-
-// kind::f16 instruction descriptor, bf16 inputs, fp32 accumulate, A K-major, B MN-major if b_mn.
-__host__ __device__ constexpr uint32_t idesc_bf16_f32_b(int M, int N, bool b_mn) {
-  return idesc_bf16_f32(M, N) | (b_mn ? (1u << 16) : 0u);
-}
-
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
@@ -75,12 +58,6 @@ struct FaParams {
   const int* q_lo;          // [B * Tq] first key each query row may see (nullptr: 0); with causal / q_pos
                             // as the last one this gives per-query key ranges (windowed attention)
 };
-
-__device__ __forceinline__ float ex2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 template <int DH>
 __global__ void __launch_bounds__(kFaThreads, 1)
@@ -373,17 +350,6 @@ __global__ void __launch_bounds__(kFaThreads, 1)
     tc_fence_after();
     tmem_dealloc(tmem, TMEM_COLS);
   }
-}
-
-// tcgen05.mma with the A operand in TMEM (P) and B from shared memory.
-__device__ __forceinline__ void umma_f16_tmem_a(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc,
-                                                uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
-      "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
-      : "memory");
 }
 
 // ------------------------------------------------------------------------------ split-row variant

@@ -1,90 +1,46 @@
-// Causal grouped-query attention over a packed batch: request b's new tokens are the rows
-// q_start[b] .. q_start[b + 1] of q, its keys the kv_len[b] rows of its cache pages (or of the packed
-// K / V rows from k_start[b]), the new tokens' own keys last:
-//   o_t = sum_j p_tj v_j / sum_j p_tj,   p_tj = exp(scale q_t . k_j - max_j),   j <= kv_len - q_len + t
-// A shared prefix of P keys (its own page list) stands in front of every request's keys and is
-// visible to every token. A row that sees no key is zero and its log-sum-exp is -inf.
-//
-// One warp per (token, head): the definition, one key at a time.
+// Packed and shared-prefix attention: argument checks, tensor maps and launches (the kernel is in
+// packed_attention_sm100.cu).
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <cudaTypedefs.h>
 
-#include "sm100_common.cuh"
+#include "packed_attention.h"
 #include "checks.h"
+#include "ops.h"
 #include "registry.h"
 
 namespace appcorr {
 
-using bf16 = __nv_bfloat16;
+// [tokens][heads][D] view of the query rows with boxes of `box_tokens` x `box_heads` x 64 columns:
+// the query heads of one key head come as consecutive shared-memory rows, token by token.
+static CUtensorMap query_tmap(const at::Tensor& q, int64_t heads, int64_t head_dim, int box_heads, int box_tokens) {
+  static PFN_cuTensorMapEncodeTiled_v12000 encode = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult r;
+    const auto st = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &r);
+    TORCH_CHECK(st == cudaSuccess && r == cudaDriverEntryPointSuccess && p != nullptr, "packed attention: cuTensorMapEncodeTiled is unavailable");
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+  }();
+  const int64_t ld = q.size(0) > 1 ? q.stride(0) : heads * head_dim;
+  CUtensorMap m;
+  cuuint64_t dims[3] = {static_cast<cuuint64_t>(head_dim), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(q.size(0))};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(head_dim * 2), static_cast<cuuint64_t>(ld * 2)};
+  cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_heads), static_cast<cuuint32_t>(box_tokens)};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = encode(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, q.data_ptr(), dims, strides, box, estr,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  APPCORR_CHECK(r == CUDA_SUCCESS, "packed attention: the query tensor map was refused: ", static_cast<int64_t>(r));
+  return m;
+}
 
-struct PaParams {
-  const bf16* q;
-  const bf16* k;
-  const bf16* v;
-  bf16* o;
-  long ldq, ldk, ldv, ldo, kv_rows;
-  const int* q_start;
-  const int* kv_len;
-  const int* table;
-  long ld_table;
-  int W;
-  const int* k_start;
-  const int* prefix;
-  int prefix_len;
-  float* lse;  // [N, H]
-  float scale;
-  int B, N, H, Hkv;
-};
-
-template <int D>
-__global__ void packed_attention_simple(PaParams p) {
-  const int n = blockIdx.x, h = blockIdx.y * blockDim.y + threadIdx.y, lane = threadIdx.x;
-  if (h >= p.H || n >= p.q_start[p.B]) return;
-  int lo = 0, hi = p.B;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (p.q_start[mid] <= n) lo = mid;
-    else hi = mid;
-  }
-  constexpr int E = D / 32;
-  const int b = lo, kvh = h / (p.H / p.Hkv);
-  float q[E], acc[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    q[e] = __bfloat162float(p.q[n * p.ldq + h * D + lane * E + e]) * p.scale;
-    acc[e] = 0.f;
-  }
-  float m = -INFINITY, l = 0.f;
-  const int own = max(p.kv_len[b] - p.q_start[b + 1] + n + 1, 0);  // own keys this token sees
-  for (int j = -p.prefix_len; j < own; ++j) {
-    long row;
-    if (j < 0 || p.table != nullptr) {
-      const int i = j < 0 ? j + p.prefix_len : j, blk = i >> 7;
-      const int page = j < 0 ? p.prefix[blk] : (blk < p.W ? p.table[b * p.ld_table + blk] : -1);
-      row = page < 0 ? -1 : (long)page * 128 + (i & 127);
-    } else {
-      row = (long)p.k_start[b] + j;
-    }
-    const bool have = row >= 0 && row < p.kv_rows;
-    float s = 0.f, vv[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      s += have ? q[e] * __bfloat162float(p.k[row * p.ldk + kvh * D + lane * E + e]) : 0.f;
-      vv[e] = have ? __bfloat162float(p.v[row * p.ldv + kvh * D + lane * E + e]) : 0.f;
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    const float mn = fmaxf(m, s), c = mn == -INFINITY ? 1.f : expf(m - mn), w = mn == -INFINITY ? 0.f : expf(s - mn);
-    m = mn;
-    l = l * c + w;
-#pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = acc[e] * c + w * vv[e];
-  }
-  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-#pragma unroll
-  for (int e = 0; e < E; ++e) p.o[n * p.ldo + h * D + lane * E + e] = __float2bfloat16_rn(acc[e] * inv);
-  if (p.lse != nullptr && lane == 0) p.lse[(long)n * p.H + h] = m + logf(l);
+// Bytes of the workspace a stream's calls share: partial results, their max and sum, arrival counters
+// (at the front; zero before the first call and between calls).
+constexpr int64_t kPaCounterBytes = 8 * sizeof(int);
+int64_t packed_attention_workspace() {
+  const int64_t blocks = packed_attention_blocks(), rows = blocks * kPaSlotsPerBlock * kPaRows;
+  return ((blocks * kPaCounterBytes + 255) / 256) * 256 + rows * (128 + 2) * sizeof(float);
 }
 
 static void pa_check_rows(const at::Tensor& t, const char* name, int64_t width) {
@@ -104,7 +60,8 @@ static void pa_check_i32(const at::Tensor& t, const char* name, int64_t dim, int
 void packed_attention_op(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, at::Tensor& o,
                          const at::Tensor& q_start, const at::Tensor& kv_len, int64_t heads, int64_t kv_heads,
                          int64_t head_dim, double scale, c10::optional<at::Tensor> table, c10::optional<at::Tensor> k_start,
-                         c10::optional<at::Tensor> prefix_table, int64_t prefix_len, c10::optional<at::Tensor> lse) {
+                         c10::optional<at::Tensor> prefix_table, int64_t prefix_len, c10::optional<at::Tensor> lse, at::Tensor& workspace,
+                         const at::Tensor& err) {
   APPCORR_CHECK(head_dim == 64 || head_dim == 128, "packed attention: head_dim must be 64 or 128, got ", head_dim);
   APPCORR_CHECK(heads > 0 && kv_heads > 0 && heads % kv_heads == 0, "packed attention: heads must be a multiple of kv_heads");
   pa_check_rows(q, "q", heads * head_dim);
@@ -138,20 +95,65 @@ void packed_attention_op(const at::Tensor& q, const at::Tensor& k, const at::Ten
     APPCORR_CHECK(t->device() == q.device(), "packed attention: tensors on different devices");
   for (auto* t : {&table, &k_start, &prefix_table, &lse})
     APPCORR_CHECK(!t->has_value() || (*t)->device() == q.device(), "packed attention: tensors on different devices");
+  APPCORR_CHECK(N < (int64_t(1) << 31) / kPaRows && k.size(0) < (int64_t(1) << 31) - 256, "packed attention: too many rows");
   if (N == 0 || B == 0) return;
-  c10::cuda::CUDAGuard guard(q.device());
-  PaParams p{reinterpret_cast<const bf16*>(q.data_ptr()), reinterpret_cast<const bf16*>(k.data_ptr()),
-             reinterpret_cast<const bf16*>(v.data_ptr()), reinterpret_cast<bf16*>(o.data_ptr()), q.stride(0), k.stride(0),
-             v.stride(0), o.stride(0), k.size(0), q_start.data_ptr<int>(), kv_len.data_ptr<int>(),
-             table.has_value() ? table->data_ptr<int>() : nullptr, table.has_value() ? table->stride(0) : 0,
-             table.has_value() ? static_cast<int>(table->size(1)) : 0, k_start.has_value() ? k_start->data_ptr<int>() : nullptr,
-             prefix_len > 0 ? prefix_table->data_ptr<int>() : nullptr, static_cast<int>(prefix_len),
-             lse.has_value() ? lse->data_ptr<float>() : nullptr, static_cast<float>(scale), static_cast<int>(B),
-             static_cast<int>(N), static_cast<int>(heads), static_cast<int>(kv_heads)};
-  dim3 grid(static_cast<unsigned>(N), static_cast<unsigned>((heads + 3) / 4));
+  APPCORR_CHECK(k.size(0) > 0, "packed attention: k and v hold no rows");
+  c10::cuda::CUDAGuard g(q.device());
+  APPCORR_CHECK(workspace.is_cuda() && workspace.scalar_type() == at::kByte && workspace.is_contiguous() &&
+                    workspace.device() == q.device() && workspace.numel() >= packed_attention_workspace(),
+                "packed attention: the workspace is too small or on another device");
+  // rows of a tile: tokens x the query heads of one key head. Groups of more than 128 heads are split evenly.
+  const int64_t group = heads / kv_heads;
+  int64_t parts = (group + 127) / 128;
+  while (group % parts) ++parts;
+  const int G = static_cast<int>(group / parts), TT = 128 / G;
+  const int64_t ldk = k.size(0) > 1 ? k.stride(0) : kv_heads * head_dim, ldv = k.size(0) > 1 ? v.stride(0) : kv_heads * head_dim;
+  const CUtensorMap tq = query_tmap(q, heads, head_dim, G, TT), tq1 = query_tmap(q, heads, head_dim, G, 1);
+  const CUtensorMap tk = make_tmap_bf16_2d(k.data_ptr(), k.size(0), kv_heads * head_dim, ldk, 128, 64);
+  const CUtensorMap tv = make_tmap_bf16_2d(v.data_ptr(), v.size(0), kv_heads * head_dim, ldv, 128, 64);
+  PackedAttnParams p{};
+  p.B = static_cast<int>(B);
+  p.N = static_cast<int>(N);
+  p.H = static_cast<int>(heads);
+  p.ng = static_cast<int>(parts);
+  p.Hv = static_cast<int>(kv_heads * parts);
+  p.G = G;
+  p.TT = TT;
+  p.q_start = q_start.data_ptr<int>();
+  p.kv_len = kv_len.data_ptr<int>();
+  p.pages = static_cast<int>(k.size(0) / 128);
+  p.key_rows = static_cast<int>(k.size(0));
+  p.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
+  p.o = reinterpret_cast<__nv_bfloat16*>(o.data_ptr());
+  p.ldo = o.size(0) > 1 ? o.stride(0) : heads * head_dim;
+  p.err = err.data_ptr<int>();
+  const int64_t blocks = packed_attention_blocks();
+  uint8_t* ws = workspace.data_ptr<uint8_t>();
+  p.counters = reinterpret_cast<int*>(ws);
+  p.slots = reinterpret_cast<float*>(ws + (blocks * kPaCounterBytes + 255) / 256 * 256);
+  p.slot_ml = p.slots + blocks * kPaSlotsPerBlock * kPaRows * 128;
   auto st = at::cuda::getCurrentCUDAStream();
-  if (head_dim == 128) packed_attention_simple<128><<<grid, dim3(32, 4), 0, st>>>(p);
-  else packed_attention_simple<64><<<grid, dim3(32, 4), 0, st>>>(p);
+  at::Tensor prior;
+  if (prefix_len > 0) {
+    prior = at::empty({N * heads, head_dim + 1}, q.options().dtype(at::kFloat));
+    p.prior = prior.data_ptr<float>();
+    p.prior_lse = p.prior + N * heads * head_dim;
+    PackedAttnParams pp = p;
+    pp.table = prefix_table->data_ptr<int>();
+    pp.W = static_cast<int>(prefix_table->numel());
+    pp.shared_len = static_cast<int>(prefix_len);
+    launch_packed_attention(static_cast<int>(head_dim), true, tq, tq1, tk, tv, pp, st);
+    C10_CUDA_KERNEL_LAUNCH_CHECK();
+  }
+  if (table.has_value()) {
+    p.table = table->data_ptr<int>();
+    p.ld_table = table->stride(0);
+    p.W = static_cast<int>(table->size(1));
+  } else {
+    p.k_start = k_start->data_ptr<int>();
+  }
+  p.lse = lse.has_value() ? lse->data_ptr<float>() : nullptr;
+  launch_packed_attention(static_cast<int>(head_dim), false, tq, tq1, tk, tv, p, st);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
@@ -159,7 +161,9 @@ void register_packed_attention_ops(pybind11::module_& m) {
   namespace py = pybind11;
   m.def("packed_attention", &packed_attention_op, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("o"), py::arg("q_start"),
         py::arg("kv_len"), py::arg("heads"), py::arg("kv_heads"), py::arg("head_dim"), py::arg("scale"), py::arg("table"),
-        py::arg("k_start"), py::arg("prefix_table"), py::arg("prefix_len"), py::arg("lse"));
+        py::arg("k_start"), py::arg("prefix_table"), py::arg("prefix_len"), py::arg("lse"),
+        py::arg("workspace"), py::arg("err"));
+  m.def("packed_attention_workspace", &packed_attention_workspace);
 }
 
 }  // namespace appcorr
