@@ -15,8 +15,6 @@ _C = None
 _IMPORT_ERROR: Exception | None = None
 _LOCK = threading.Lock()
 _ERR_WORDS: dict[int, torch.Tensor] = {}
-# called (no arguments) after check_errors found an error: drop state that an abandoned kernel may have left
-ERROR_HOOKS: list = []
 
 ERROR_NAMES = {
     0: "ok",
@@ -72,6 +70,4 @@ def check_errors(device: torch.device | None = None) -> None:
         code = int(w.item())
         if code != 0:
             w.zero_()
-            for hook in ERROR_HOOKS:
-                hook()
             raise RuntimeError(f"appcorr_b200 kernel error on {d}: {ERROR_NAMES.get(code, code)}")

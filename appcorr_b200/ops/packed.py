@@ -17,34 +17,20 @@ as a key it reads as a row of zeros.
 """
 from __future__ import annotations
 
-from typing import Dict, Optional, Tuple
+from typing import Optional
 
 import torch
 
 from .kernels import _count
-from .native import ERROR_HOOKS, err_word, lib
+from .native import err_word, lib
 
 PAGE = 128  # rows per K/V cache page
 
-# Partial results of rows whose keys are split over SMs, one workspace (39 MB) per device and stream:
-# calls on one stream follow each other, calls on several streams keep apart.
-_WORKSPACES: Dict[Tuple[int, int], torch.Tensor] = {}
 
-
-def _workspace(device: torch.device) -> torch.Tensor:
-    if device.type != "cuda":
-        raise RuntimeError(f"packed attention: q must be a CUDA tensor, got one on {device}")
-    key = (device.index, torch.cuda.current_stream(device).cuda_stream)
-    w = _WORKSPACES.get(key)
-    if w is None:
-        with torch.cuda.device(device):
-            w = torch.zeros(lib().packed_attention_workspace(), dtype=torch.uint8, device=device)
-        _WORKSPACES[key] = w
-    return w
-
-
-# a kernel that gave up a wait may leave arrival counters behind: the next calls start from fresh ones
-ERROR_HOOKS.append(_WORKSPACES.clear)
+def _err(q: torch.Tensor) -> torch.Tensor:
+    if q.device.type != "cuda":
+        raise RuntimeError(f"packed attention: q must be a CUDA tensor, got one on {q.device}")
+    return err_word(q.device)
 
 
 def packed_layout(q_len: torch.Tensor, past: torch.Tensor, table: torch.Tensor, free_pages: torch.Tensor,
@@ -91,9 +77,9 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch
     kv_len[b] packed rows of k / v from k_start[b]. Rows past q_start[B] are not touched; a token
     that sees no key gets zeros (lse -inf). Cached rows past kv_len may hold anything. lse: fp32
     [N, heads] natural log-sum-exp of the scaled scores. scale: head_dim ** -0.5 by default."""
-    _count()
+    _count(2)
     lib().packed_attention(q, k, v, o, q_start, kv_len, heads, kv_heads, head_dim,
-                           head_dim ** -0.5 if scale is None else scale, table, k_start, None, 0, lse, _workspace(q.device), err_word(q.device))
+                           head_dim ** -0.5 if scale is None else scale, table, k_start, None, 0, lse, _err(q))
     return o
 
 
@@ -105,8 +91,7 @@ def shared_prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o
     (pages prefix_table [>= ceil(prefix_len / 128)] of the same pools) are visible to every token, in
     front of the request's own kv_len[b] keys, which are paged through `table` and causal as there.
     kv_len counts a request's own keys only and may be zero."""
-    _count(2 if prefix_len else 1)
+    _count(2)
     lib().packed_attention(q, k, v, o, q_start, kv_len, heads, kv_heads, head_dim,
-                           head_dim ** -0.5 if scale is None else scale, table, None, prefix_table, prefix_len, lse, _workspace(q.device),
-                           err_word(q.device))
+                           head_dim ** -0.5 if scale is None else scale, table, None, prefix_table, prefix_len, lse, _err(q))
     return o

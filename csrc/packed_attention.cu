@@ -35,14 +35,6 @@ static CUtensorMap query_tmap(const at::Tensor& q, int64_t heads, int64_t head_d
   return m;
 }
 
-// Bytes of the workspace a stream's calls share: partial results, their max and sum, arrival counters
-// (at the front; zero before the first call and between calls).
-constexpr int64_t kPaCounterBytes = 8 * sizeof(int);
-int64_t packed_attention_workspace() {
-  const int64_t blocks = packed_attention_blocks(), rows = blocks * kPaSlotsPerBlock * kPaRows;
-  return ((blocks * kPaCounterBytes + 255) / 256) * 256 + rows * (128 + 2) * sizeof(float);
-}
-
 static void pa_check_rows(const at::Tensor& t, const char* name, int64_t width) {
   APPCORR_CHECK(t.is_cuda() && t.scalar_type() == at::kBFloat16 && t.dim() == 2 && t.stride(1) == 1, "packed attention: ", name,
               " must be a 2-D CUDA bf16 tensor with unit inner stride");
@@ -60,8 +52,7 @@ static void pa_check_i32(const at::Tensor& t, const char* name, int64_t dim, int
 void packed_attention_op(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, at::Tensor& o,
                          const at::Tensor& q_start, const at::Tensor& kv_len, int64_t heads, int64_t kv_heads,
                          int64_t head_dim, double scale, c10::optional<at::Tensor> table, c10::optional<at::Tensor> k_start,
-                         c10::optional<at::Tensor> prefix_table, int64_t prefix_len, c10::optional<at::Tensor> lse, at::Tensor& workspace,
-                         const at::Tensor& err) {
+                         c10::optional<at::Tensor> prefix_table, int64_t prefix_len, c10::optional<at::Tensor> lse, const at::Tensor& err) {
   APPCORR_CHECK(head_dim == 64 || head_dim == 128, "packed attention: head_dim must be 64 or 128, got ", head_dim);
   APPCORR_CHECK(heads > 0 && kv_heads > 0 && heads % kv_heads == 0, "packed attention: heads must be a multiple of kv_heads");
   pa_check_rows(q, "q", heads * head_dim);
@@ -99,9 +90,6 @@ void packed_attention_op(const at::Tensor& q, const at::Tensor& k, const at::Ten
   if (N == 0 || B == 0) return;
   APPCORR_CHECK(k.size(0) > 0, "packed attention: k and v hold no rows");
   c10::cuda::CUDAGuard g(q.device());
-  APPCORR_CHECK(workspace.is_cuda() && workspace.scalar_type() == at::kByte && workspace.is_contiguous() &&
-                    workspace.device() == q.device() && workspace.numel() >= packed_attention_workspace(),
-                "packed attention: the workspace is too small or on another device");
   // rows of a tile: tokens x the query heads of one key head. Groups of more than 128 heads are split evenly.
   const int64_t group = heads / kv_heads;
   int64_t parts = (group + 127) / 128;
@@ -127,24 +115,6 @@ void packed_attention_op(const at::Tensor& q, const at::Tensor& k, const at::Ten
   p.o = reinterpret_cast<__nv_bfloat16*>(o.data_ptr());
   p.ldo = o.size(0) > 1 ? o.stride(0) : heads * head_dim;
   p.err = err.data_ptr<int>();
-  const int64_t blocks = packed_attention_blocks();
-  uint8_t* ws = workspace.data_ptr<uint8_t>();
-  p.counters = reinterpret_cast<int*>(ws);
-  p.slots = reinterpret_cast<float*>(ws + (blocks * kPaCounterBytes + 255) / 256 * 256);
-  p.slot_ml = p.slots + blocks * kPaSlotsPerBlock * kPaRows * 128;
-  auto st = at::cuda::getCurrentCUDAStream();
-  at::Tensor prior;
-  if (prefix_len > 0) {
-    prior = at::empty({N * heads, head_dim + 1}, q.options().dtype(at::kFloat));
-    p.prior = prior.data_ptr<float>();
-    p.prior_lse = p.prior + N * heads * head_dim;
-    PackedAttnParams pp = p;
-    pp.table = prefix_table->data_ptr<int>();
-    pp.W = static_cast<int>(prefix_table->numel());
-    pp.shared_len = static_cast<int>(prefix_len);
-    launch_packed_attention(static_cast<int>(head_dim), true, tq, tq1, tk, tv, pp, st);
-    C10_CUDA_KERNEL_LAUNCH_CHECK();
-  }
   if (table.has_value()) {
     p.table = table->data_ptr<int>();
     p.ld_table = table->stride(0);
@@ -153,7 +123,22 @@ void packed_attention_op(const at::Tensor& q, const at::Tensor& k, const at::Ten
     p.k_start = k_start->data_ptr<int>();
   }
   p.lse = lse.has_value() ? lse->data_ptr<float>() : nullptr;
-  launch_packed_attention(static_cast<int>(head_dim), false, tq, tq1, tk, tv, p, st);
+  // room for partial results: from the caching allocator, so calls on different streams keep apart
+  const int64_t blocks = packed_attention_blocks(), slot_rows = blocks * kPaSlotsPerBlock * kPaRows;
+  const int64_t row_words = prefix_len > 0 ? 2 * N * heads * (head_dim + 3) : 0;
+  at::Tensor room = at::empty({slot_rows * (head_dim + 2) + blocks * 4 + row_words}, q.options().dtype(at::kFloat));
+  p.slots = room.data_ptr<float>();
+  p.slot_ml = p.slots + slot_rows * head_dim;
+  p.cuts = reinterpret_cast<CutTile*>(p.slot_ml + slot_rows * 2);
+  if (prefix_len > 0) {
+    p.prefix = prefix_table->data_ptr<int>();
+    p.prefix_pages = static_cast<int>(prefix_table->numel());
+    p.shared_len = static_cast<int>(prefix_len);
+    p.row_o = reinterpret_cast<float*>(p.cuts + blocks);
+    p.row_ml = p.row_o + 2 * N * heads * head_dim;
+    p.row_parts = reinterpret_cast<int*>(p.row_ml + 4 * N * heads);
+  }
+  launch_packed_attention(static_cast<int>(head_dim), tq, tq1, tk, tv, p, at::cuda::getCurrentCUDAStream());
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
@@ -162,8 +147,7 @@ void register_packed_attention_ops(pybind11::module_& m) {
   m.def("packed_attention", &packed_attention_op, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("o"), py::arg("q_start"),
         py::arg("kv_len"), py::arg("heads"), py::arg("kv_heads"), py::arg("head_dim"), py::arg("scale"), py::arg("table"),
         py::arg("k_start"), py::arg("prefix_table"), py::arg("prefix_len"), py::arg("lse"),
-        py::arg("workspace"), py::arg("err"));
-  m.def("packed_attention_workspace", &packed_attention_workspace);
+        py::arg("err"));
 }
 
 }  // namespace appcorr
