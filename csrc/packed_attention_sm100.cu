@@ -63,6 +63,12 @@ struct Cfg {
 
 enum : int { kWhole = 1, kEnd = 2, kAlt = 4, kShared = 8 };
 
+// shared-memory descriptors without their address (bits 0..13, address / 16)
+constexpr uint64_t sw128_kmajor_desc_base() { return 1ull << 16 | (1024ull >> 4) << 32 | 1ull << 46 | 2ull << 61; }
+constexpr uint64_t sw128_mnmajor_desc_base(uint32_t lbo, uint32_t sbo) {
+  return static_cast<uint64_t>(lbo >> 4) << 16 | static_cast<uint64_t>(sbo >> 4) << 32 | 1ull << 46 | 2ull << 61;
+}
+
 struct Tile {
   int tok0, ntok;  // first packed row and number of tokens
   int lim0;        // last key visible to its first token
@@ -120,8 +126,67 @@ __device__ __forceinline__ int cut_block(long w, long at, long cost, int nb) {
 }
 __device__ __forceinline__ long stretch(long W, int c, int n) { return W * c / n; }
 
+// Bounded wait of a whole warp. It polls without reading a clock: the waits lie on the chain of
+// S, softmax, P V, and a wait that reads the global timer as soon as its first poll fails (as
+// mbar_wait does) took 2.4 us for a key block where 1.1 us of products are done. 2^22 polls, each of
+// which the hardware may suspend for a while, are tenths of a second at the least; tiles take less than
+// a millisecond.
+__device__ __forceinline__ bool poll(uint32_t bar, uint32_t parity, int* err, int code) {
+#pragma unroll 1
+  for (int i = 0; i < (1 << 22); ++i) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((i & 1023) == 1023 && error_raised(err)) return false;
+  }
+  record_error(err, code);
+  return false;
+}
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, int* err, int code) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, code));
+  return __all_sync(0xffffffffu, poll(bar, parity, err, code));
+}
+
+// MMA and commit by one elected lane of a warp whose control flow is uniform. The election sits
+// inside the instruction's own predicate: under an `if (lane == 0)` the operands of every MMA are moved
+// to uniform registers one by one and the issue of 8 MMAs (512 clocks of work) takes 460 clocks, this
+// way 310, so that the tensor core's queue stays ahead of the waits in between.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// two floats of one 64-bit register pair at a time
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
 }
 
 template <int DH>
@@ -423,16 +488,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       int np_[2] = {0, 0}, no_[2] = {0, 0};  // P tiles and O tiles consumed per half
       const uint32_t qa = smem_addr(sQ), kva = smem_addr(sKV);
       auto landed = [&](uint32_t i) { return warp_wait(smem_addr(&full[i % NST]), (i / NST) & 1, p.err, kErrTimeoutMma); };
+      constexpr uint64_t kDescK = sw128_kmajor_desc_base(), kDescV = sw128_mnmajor_desc_base(C::CHUNK, 1024);
       auto issue_s = [&](int hf, int qh, uint32_t i) {  // S of half hf from Q half qh and ring entry i
-        if (lane == 0) {
-          const uint32_t ka = kva + (i % NST) * C::TILE, qb = qa + qh * C::TILE;
+        const uint64_t ka = kDescK | ((kva + (i % NST) * C::TILE) >> 4), qb = kDescK | ((qa + qh * C::TILE) >> 4);
 #pragma unroll
-          for (int k = 0; k < DH / 16; ++k) {
-            const uint32_t off = (k >> 2) * C::CHUNK + (k & 3) * 32;
-            umma_f16(tmem + hf * 128, sw128_kmajor_desc(qb + off), sw128_kmajor_desc(ka + off), IDESC_S, k > 0);
-          }
-          umma_commit(smem_addr(&s_full[hf]));
+        for (int k = 0; k < DH / 16; ++k) {
+          const uint32_t off = ((k >> 2) * C::CHUNK + (k & 3) * 32) >> 4;
+          mma_ss(tmem + hf * 128, qb + off, ka + off, IDESC_S, k > 0);
         }
+        mma_commit(smem_addr(&s_full[hf]));
       };
       // V rows of keys that do not exist become zeros; `live` of the 128 exist
       auto clear_dead = [&](uint32_t i, int live) {
@@ -452,21 +516,21 @@ __global__ void __launch_bounds__(kThreads, 1)
           ++no_[hf];
         }
         tc_fence_after();
-        if (lane == 0) {
-          const uint32_t va = kva + (i % NST) * C::TILE;
+        const uint64_t va = kDescV | ((kva + (i % NST) * C::TILE) >> 4);
 #pragma unroll
-          for (int k = 0; k < kBlk / 16; ++k)
-            umma_f16_tmem_a(tmem + O_COL + hf * 128, tmem + hf * 128 + k * 8, sw128_mnmajor_desc(va + k * 2048, C::CHUNK, 1024),
-                            IDESC_O, (!first || k > 0) ? 1u : 0u);
-          if (last) umma_commit(smem_addr(&o_full[hf]));
-        }
+        for (int k = 0; k < kBlk / 16; ++k)
+          mma_ts(tmem + O_COL + hf * 128, tmem + hf * 128 + k * 8, va + k * (2048 >> 4), IDESC_O, (!first || k > 0) ? 1u : 0u);
+        if (last) mma_commit(smem_addr(&o_full[hf]));
         return true;
       };
       for (int np = 0;; ++np) {
         ok = warp_wait(smem_addr(&t_full[np % kTiles]), (np / kTiles) & 1, p.err, kErrTimeoutMma);
         if (!ok) break;
         const Tile& tl = tiles[np % kTiles];
-        const int flags = tl.flags, n0 = tl.n0, n1 = tl.n1, kv = tl.kv, jb = tl.jb;
+        // broadcast, so that the compiler keeps the loops below uniform
+        const int flags = __shfl_sync(0xffffffffu, tl.flags, 0), n0 = __shfl_sync(0xffffffffu, tl.n0, 0),
+                  n1 = __shfl_sync(0xffffffffu, tl.n1, 0), kv = __shfl_sync(0xffffffffu, tl.kv, 0),
+                  jb = __shfl_sync(0xffffffffu, tl.jb, 0);
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_addr(&t_empty[np % kTiles]));
         if (flags & kEnd) break;
@@ -480,15 +544,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           // block j in half j & 1: S_0 S_1, then PV_j S_{j+2}; ring entries 2j (K), 2j + 1 (V)
           const uint32_t i0 = it;
           issue_s(0, 0, i0);
-          if (lane == 0) umma_commit(smem_addr(&empty[i0 % NST]));
+          mma_commit(smem_addr(&empty[i0 % NST]));
           ok = landed(i0 + 2);
           if (!ok) break;
           tc_fence_after();
           issue_s(1, 0, i0 + 2);
-          if (lane == 0) {
-            umma_commit(smem_addr(&empty[(i0 + 2) % NST]));
-            if (cnt == 2) umma_commit(smem_addr(q_empty));
-          }
+          mma_commit(smem_addr(&empty[(i0 + 2) % NST]));
+          if (cnt == 2) mma_commit(smem_addr(q_empty));
           for (int j = 0; ok && j < cnt; ++j) {
             const uint32_t iv = i0 + 2 * j + 1, ik = iv + 3;
             ok = landed(iv);
@@ -496,26 +558,22 @@ __global__ void __launch_bounds__(kThreads, 1)
             clear_dead(iv, kv - (jb + j) * kBlk);
             ok = issue_pv(j & 1, iv, j < 2, j + 2 >= cnt);
             if (!ok) break;
-            if (lane == 0) umma_commit(smem_addr(&empty[iv % NST]));
+            mma_commit(smem_addr(&empty[iv % NST]));
             if (j + 2 < cnt) {
               ok = landed(ik);
               if (!ok) break;
               tc_fence_after();
               issue_s(j & 1, 0, ik);
-              if (lane == 0) {
-                umma_commit(smem_addr(&empty[ik % NST]));
-                if (j + 3 == cnt) umma_commit(smem_addr(q_empty));
-              }
+              mma_commit(smem_addr(&empty[ik % NST]));
+              if (j + 3 == cnt) mma_commit(smem_addr(q_empty));
             }
           }
           it = i0 + 2 * cnt;
         } else {
           if (n0 > 0) issue_s(0, 0, it);
           if (n1 > 0) issue_s(1, 1, it);
-          if (lane == 0) {
-            umma_commit(smem_addr(&empty[it % NST]));
-            if (cnt == 1) umma_commit(smem_addr(q_empty));
-          }
+          mma_commit(smem_addr(&empty[it % NST]));
+          if (cnt == 1) mma_commit(smem_addr(q_empty));
           ++it;
           for (int j = 0; ok && j < cnt; ++j) {
             const uint32_t iv = it, ik = it + 1;
@@ -534,12 +592,10 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (j + 1 < nh) issue_s(hf, hf, ik);
             }
             if (!ok) break;
-            if (lane == 0) {
-              umma_commit(smem_addr(&empty[iv % NST]));
-              if (more) {
-                umma_commit(smem_addr(&empty[ik % NST]));
-                if (j + 2 == cnt) umma_commit(smem_addr(q_empty));
-              }
+            mma_commit(smem_addr(&empty[iv % NST]));
+            if (more) {
+              mma_commit(smem_addr(&empty[ik % NST]));
+              if (j + 2 == cnt) mma_commit(smem_addr(q_empty));
             }
             it += more ? 2 : 1;
           }
@@ -547,7 +603,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
       }
       if (!ok) {  // products in flight end before TMEM is given back
-        if (lane == 0) umma_commit(smem_addr(done));
+        mma_commit(smem_addr(done));
         mbar_wait(smem_addr(done), 0, nullptr, 0);
       }
     }
@@ -599,8 +655,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           float mx[4] = {sv[0], sv[1], sv[2], sv[3]};
 #pragma unroll
-          for (int i = 4; i < kBlk; ++i) mx[i & 3] = fmaxf(mx[i & 3], sv[i]);
-          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          for (int i = 4; i < kBlk; i += 8) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              if (i + 2 * u + 1 < kBlk) mx[u] = max3(mx[u], sv[i + 2 * u], sv[i + 2 * u + 1]);
+          }
+          const float top = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]);
           const bool grow = valid && (top - m_run) * sl2 > 8.f;
           float corr = 1.f;
           if (grow) {
@@ -620,21 +680,25 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
           const float moff = m_run == -INFINITY ? 0.f : m_run * sl2;
-          float ls[4] = {0.f, 0.f, 0.f, 0.f};
+          const uint64_t sl2x2 = pack2(sl2, sl2), offx2 = pack2(-moff, -moff);
+          uint64_t ls[2] = {0, 0};
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             uint32_t pk[32];
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
-              const float e0 = ex2_approx(fmaf(sv[c * 64 + 2 * i], sl2, -moff));
-              const float e1 = ex2_approx(fmaf(sv[c * 64 + 2 * i + 1], sl2, -moff));
-              ls[(2 * i) & 3] += e0;
-              ls[(2 * i + 1) & 3] += e1;
+              float e0, e1;
+              unpack2(fma2(pack2(sv[c * 64 + 2 * i], sv[c * 64 + 2 * i + 1]), sl2x2, offx2), e0, e1);
+              e0 = ex2_approx(e0);
+              e1 = ex2_approx(e1);
+              ls[i & 1] = add2(ls[i & 1], pack2(e0, e1));
               pk[i] = pack_bf16x2(e0, e1);
             }
             tmem_st32(s_addr + c * 32, pk);
           }
-          l_run += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+          float l0, l1;
+          unpack2(add2(ls[0], ls[1]), l0, l1);
+          l_run += l0 + l1;
           tmem_wait_st();
         }
         tc_fence_before();
