@@ -47,7 +47,7 @@ constexpr int kThreads = 384;      // three warpgroups: roles, softmax of half 0
 constexpr int kMaxBlocks = 256;    // blocks of a launch (one per SM)
 constexpr int kTiles = 4;          // published tiles in flight
 constexpr int kBlk = 128;          // keys per block = rows per page
-constexpr long kTileCost = 128;    // a tile's fixed cost, in keys
+constexpr long kTileCost = 256;    // a tile's fixed cost, in keys (3.4 us beside 2.1 us for a key block of two halves)
 constexpr long kLeastWork = 128;   // least stretch of a block: at least one block boundary lies in it,
                                    // so the blocks that share a tile's keys are consecutive
 
@@ -142,6 +142,12 @@ __device__ __forceinline__ bool poll(uint32_t bar, uint32_t parity, int* err, in
 }
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, int* err, int code) {
   return __all_sync(0xffffffffu, poll(bar, parity, err, code));
+}
+// two barriers at once: one latency where both are done
+__device__ __forceinline__ bool warp_wait2(uint32_t bar0, uint32_t parity0, uint32_t bar1, uint32_t parity1, int* err, int code) {
+  const bool d0 = mbar_try_wait(bar0, parity0), d1 = mbar_try_wait(bar1, parity1);
+  if (__all_sync(0xffffffffu, d0 && d1)) return true;
+  return warp_wait(bar0, parity0, err, code) && warp_wait(bar1, parity1, err, code);
 }
 
 // MMA and commit by one elected lane of a warp whose control flow is uniform. The election sits
@@ -578,11 +584,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int j = 0; ok && j < cnt; ++j) {
             const uint32_t iv = it, ik = it + 1;
             const bool more = j + 1 < cnt;
-            ok = landed(iv);
+            ok = more ? warp_wait2(smem_addr(&full[iv % NST]), (iv / NST) & 1, smem_addr(&full[ik % NST]), (ik / NST) & 1, p.err, kErrTimeoutMma)
+                      : landed(iv);
             if (!ok) break;
             clear_dead(iv, kv - (jb + j) * kBlk);
-            if (more) ok = landed(ik);
-            if (!ok) break;
 #pragma unroll
             for (int hf = 0; hf < 2; ++hf) {
               const int nh = hf ? n1 : n0;
@@ -765,41 +770,37 @@ __global__ void __launch_bounds__(kThreads, 1)
       const long tok = tl.tok0 + tk;
       const int head = tl.hv * p.G + rhead;
       const long orow = tok * p.H + head;
-      auto load_o = [&](int c, float (&x)[32]) {  // 32 columns of this row's O (both halves' of a kAlt tile)
-        uint32_t u[32];
-        __syncwarp();
-        if (cnt > 0) {
-          tmem_ld32(o_addr + c * 32, u);
-          tmem_wait_ld();
-        } else {
+      // this row's O (both halves' of a kAlt tile) comes to registers whole, so that the next tile's
+      // products may start before it is stored
+      float x[DH];
+      if (cnt > 0) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) u[i] = 0u;
-        }
+        for (int c = 0; c < DH / 32; ++c) tmem_ld32(o_addr + c * 32, *reinterpret_cast<uint32_t(*)[32]>(reinterpret_cast<uint32_t*>(x) + c * 32));
+        tmem_wait_ld();
+      } else {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(u[i]);
-        if (alt) {
+        for (int i = 0; i < DH; ++i) x[i] = 0.f;
+      }
+      if (alt) {
+#pragma unroll
+        for (int c = 0; c < DH / 32; ++c) {
+          uint32_t u[32];
           tmem_ld32(o_addr + 128 + c * 32, u);
           tmem_wait_ld();
 #pragma unroll
-          for (int i = 0; i < 32; ++i) x[i] = x[i] * a0 + __uint_as_float(u[i]) * a1;
+          for (int i = 0; i < 32; ++i) x[c * 32 + i] = x[c * 32 + i] * a0 + __uint_as_float(u[i]) * a1;
         }
-      };
-      if ((flags & kWhole) && p.row_o == nullptr) {  // the tile's only part: the result
+      }
+      o_done();
+      if (!valid) {
+      } else if ((flags & kWhole) && p.row_o == nullptr) {  // the tile's only part: the result
         const float inv = l_run > 0.f || l_run != l_run ? 1.f / l_run : 0.f;
-#pragma unroll 1
-        for (int c = 0; c < DH / 32; ++c) {
-          float x[32];
-          load_o(c, x);
-          if (valid) {
-            uint4* dst = reinterpret_cast<uint4*>(p.o + tok * p.ldo + (long)head * DH + c * 32);
+        uint4* dst = reinterpret_cast<uint4*>(p.o + tok * p.ldo + (long)head * DH);
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              dst[i] = make_uint4(pack_bf16x2(x[8 * i] * inv, x[8 * i + 1] * inv), pack_bf16x2(x[8 * i + 2] * inv, x[8 * i + 3] * inv),
-                                  pack_bf16x2(x[8 * i + 4] * inv, x[8 * i + 5] * inv), pack_bf16x2(x[8 * i + 6] * inv, x[8 * i + 7] * inv));
-          }
-        }
-        o_done();
-        if (valid && p.lse != nullptr) p.lse[orow] = (mlog + log2f(l_run)) * 0.69314718055994531f;
+        for (int i = 0; i < DH / 8; ++i)
+          dst[i] = make_uint4(pack_bf16x2(x[8 * i] * inv, x[8 * i + 1] * inv), pack_bf16x2(x[8 * i + 2] * inv, x[8 * i + 3] * inv),
+                              pack_bf16x2(x[8 * i + 4] * inv, x[8 * i + 5] * inv), pack_bf16x2(x[8 * i + 6] * inv, x[8 * i + 7] * inv));
+        if (p.lse != nullptr) p.lse[orow] = (mlog + log2f(l_run)) * 0.69314718055994531f;
       } else {  // a part: O, maximum and sum for the joining kernel
         const long cls = flags & kShared ? (long)p.N * p.H : 0;
         float *dst_o, *dst_ml;
@@ -811,21 +812,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           dst_o = p.slots + srow * DH;
           dst_ml = p.slot_ml + srow * 2;
         }
-#pragma unroll 1
-        for (int c = 0; c < DH / 32; ++c) {
-          float x[32];
-          load_o(c, x);
-          if (valid) {
-            float4* dst = reinterpret_cast<float4*>(dst_o + c * 32);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) dst[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
-          }
-        }
-        o_done();
-        if (valid) {
-          *reinterpret_cast<float2*>(dst_ml) = make_float2(mlog, l_run);
-          if (p.row_o != nullptr) p.row_parts[cls + orow] = flags & kWhole ? -1 : tl.parts;
-        }
+        for (int i = 0; i < DH / 4; ++i)
+          reinterpret_cast<float4*>(dst_o)[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+        *reinterpret_cast<float2*>(dst_ml) = make_float2(mlog, l_run);
+        if (p.row_o != nullptr) p.row_parts[cls + orow] = flags & kWhole ? -1 : tl.parts;
       }
       release();
     }
