@@ -36,6 +36,9 @@
 // All waits are bounded; a wait that runs out sets the error word and every role leaves.
 #include "packed_attention.h"
 
+#include <atomic>
+#include <type_traits>
+
 #include "sm100_common.cuh"
 
 namespace appcorr {
@@ -126,6 +129,11 @@ __device__ __forceinline__ int cut_block(long w, long at, long cost, int nb) {
 }
 __device__ __forceinline__ long stretch(long W, int c, int n) { return W * c / n; }
 
+// Programmatic dependent launch: a kernel of this file starts while the one before it ends, and waits
+// here before it touches what that one (or any before it) wrote.
+__device__ __forceinline__ void wait_for_earlier_kernels() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_later_kernels_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // Bounded wait of a whole warp. It polls without reading a clock: the waits lie on the chain of
 // S, softmax, P V, and a wait that reads the global timer as soon as its first poll fails (as
 // mbar_wait does) took 2.4 us for a key block where 1.1 us of products are done. 2^22 polls, each of
@@ -193,6 +201,30 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
+}
+
+// 16 TMEM lanes x 64 columns: register 4 g + e of a thread holds row lane / 4 (+ 8 for e >= 2) and
+// column 8 g + 2 (lane % 4) + (e & 1)
+__device__ __forceinline__ void tmem_ld_16x64(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+// 4 x 4 transposition inside a quad of lanes: register i of lane q becomes register q of lane i
+__device__ __forceinline__ void quad_transpose(uint32_t (&r)[4], int q) {
+#pragma unroll
+  for (int i = 0; i < 4; i += 2) {
+    const uint32_t w = __shfl_xor_sync(0xffffffffu, q & 1 ? r[i] : r[i + 1], 1);
+    if (q & 1) r[i] = w;
+    else r[i + 1] = w;
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t w = __shfl_xor_sync(0xffffffffu, q & 2 ? r[i] : r[i + 2], 2);
+    if (q & 2) r[i] = w;
+    else r[i + 2] = w;
+  }
 }
 
 template <int DH>
@@ -265,6 +297,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     tmem_alloc(smem_addr(&s_int[1]), 512);
     tmem_relinquish();
   }
+
+  wait_for_earlier_kernels();
+  let_later_kernels_start();
 
   // ---------------------------------------------------------------- this block's stretch of the line
   const int E = p.B + (p.shared_len > 0);
@@ -770,53 +805,95 @@ __global__ void __launch_bounds__(kThreads, 1)
       const long tok = tl.tok0 + tk;
       const int head = tl.hv * p.G + rhead;
       const long orow = tok * p.H + head;
-      // this row's O (both halves' of a kAlt tile) comes to registers whole, so that the next tile's
-      // products may start before it is stored
-      float x[DH];
-      if (cnt > 0) {
+      // O goes out 16 rows x 64 columns at a time, in an order in which a quad of lanes holds 64 bytes of
+      // a row (with a row per lane every store touches 32 rows). The loops stay rolled: this code runs
+      // once per tile, and unrolled it spent 4000 clocks and more on fetching instructions.
+      const int q4 = lane & 3;
+      auto load_o = [&](int h, int c, uint32_t (&x)[32]) {  // rows 16 h .. 16 h + 15, columns 64 c .. 64 c + 63
+        __syncwarp();
+        if (cnt > 0) {
+          tmem_ld_16x64(o_addr + (h << 20) + c * 64, x);
+          tmem_wait_ld();
+        } else {
 #pragma unroll
-        for (int c = 0; c < DH / 32; ++c) tmem_ld32(o_addr + c * 32, *reinterpret_cast<uint32_t(*)[32]>(reinterpret_cast<uint32_t*>(x) + c * 32));
-        tmem_wait_ld();
-      } else {
-#pragma unroll
-        for (int i = 0; i < DH; ++i) x[i] = 0.f;
-      }
-      if (alt) {
-#pragma unroll
-        for (int c = 0; c < DH / 32; ++c) {
+          for (int i = 0; i < 32; ++i) x[i] = 0u;
+        }
+        if (alt) {  // and half 1's accumulators of the same rows
           uint32_t u[32];
-          tmem_ld32(o_addr + 128 + c * 32, u);
+          tmem_ld_16x64(o_addr + 128 + (h << 20) + c * 64, u);
+          const int r0 = 16 * h + lane / 4;
+          const float f0 = __shfl_sync(0xffffffffu, a0, r0), f1 = __shfl_sync(0xffffffffu, a1, r0);
+          const float g0 = __shfl_sync(0xffffffffu, a0, r0 + 8), g1 = __shfl_sync(0xffffffffu, a1, r0 + 8);
           tmem_wait_ld();
 #pragma unroll
-          for (int i = 0; i < 32; ++i) x[c * 32 + i] = x[c * 32 + i] * a0 + __uint_as_float(u[i]) * a1;
+          for (int i = 0; i < 32; ++i)
+            x[i] = __float_as_uint(__uint_as_float(x[i]) * (i & 2 ? g0 : f0) + __uint_as_float(u[i]) * (i & 2 ? g1 : f1));
         }
-      }
-      o_done();
-      if (!valid) {
-      } else if ((flags & kWhole) && p.row_o == nullptr) {  // the tile's only part: the result
+      };
+      const unsigned stored = __ballot_sync(0xffffffffu, valid);
+      if ((flags & kWhole) && p.row_o == nullptr) {  // the tile's only part: the result
         const float inv = l_run > 0.f || l_run != l_run ? 1.f / l_run : 0.f;
-        uint4* dst = reinterpret_cast<uint4*>(p.o + tok * p.ldo + (long)head * DH);
+        const long at = tok * p.ldo + (long)head * DH;
+#pragma unroll 1
+        for (int hc = 0; hc < DH / 32; ++hc) {
+          const int h = hc & 1, c = hc >> 1;
+          if (!((stored >> (16 * h)) & 0xFFFFu)) continue;
+          uint32_t x[32];
+          load_o(h, c, x);
 #pragma unroll
-        for (int i = 0; i < DH / 8; ++i)
-          dst[i] = make_uint4(pack_bf16x2(x[8 * i] * inv, x[8 * i + 1] * inv), pack_bf16x2(x[8 * i + 2] * inv, x[8 * i + 3] * inv),
-                              pack_bf16x2(x[8 * i + 4] * inv, x[8 * i + 5] * inv), pack_bf16x2(x[8 * i + 6] * inv, x[8 * i + 7] * inv));
-        if (p.lse != nullptr) p.lse[orow] = (mlog + log2f(l_run)) * 0.69314718055994531f;
+          for (int k = 0; k < 2; ++k) {  // rows lane / 4 and lane / 4 + 8 of the 16
+            const int r = 16 * h + 8 * k + lane / 4;
+            const float w = __shfl_sync(0xffffffffu, inv, r);
+            bf16* dst = p.o + __shfl_sync(0xffffffffu, at, r) + c * 64 + q4 * 8;
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+              uint32_t v[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int e = (4 * b + i) * 4 + k * 2;
+                v[i] = pack_bf16x2(__uint_as_float(x[e]) * w, __uint_as_float(x[e + 1]) * w);
+              }
+              quad_transpose(v, q4);
+              if ((stored >> r) & 1) *reinterpret_cast<uint4*>(dst + b * 32) = make_uint4(v[0], v[1], v[2], v[3]);
+            }
+          }
+        }
+        o_done();
+        if (valid && p.lse != nullptr) p.lse[orow] = (mlog + log2f(l_run)) * 0.69314718055994531f;
       } else {  // a part: O, maximum and sum for the joining kernel
         const long cls = flags & kShared ? (long)p.N * p.H : 0;
-        float *dst_o, *dst_ml;
-        if (flags & kWhole) {
-          dst_o = p.row_o + (cls + orow) * DH;
-          dst_ml = p.row_ml + (cls + orow) * 2;
-        } else {
-          const long srow = (long)tl.slot * kPaRows + (alt ? 0 : hf * 128) + row;
-          dst_o = p.slots + srow * DH;
-          dst_ml = p.slot_ml + srow * 2;
-        }
+        const long prow = flags & kWhole ? cls + orow : (long)tl.slot * kPaRows + (alt ? 0 : hf * 128) + row;
+        float* part_o = flags & kWhole ? p.row_o : p.slots;
+        float* part_ml = flags & kWhole ? p.row_ml : p.slot_ml;
+#pragma unroll 1
+        for (int hc = 0; hc < DH / 32; ++hc) {
+          const int h = hc & 1, c = hc >> 1;
+          if (!((stored >> (16 * h)) & 0xFFFFu)) continue;
+          uint32_t x[32];
+          load_o(h, c, x);
 #pragma unroll
-        for (int i = 0; i < DH / 4; ++i)
-          reinterpret_cast<float4*>(dst_o)[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
-        *reinterpret_cast<float2*>(dst_ml) = make_float2(mlog, l_run);
-        if (p.row_o != nullptr) p.row_parts[cls + orow] = flags & kWhole ? -1 : tl.parts;
+          for (int k = 0; k < 2; ++k) {
+            const int r = 16 * h + 8 * k + lane / 4;
+            float* dst = part_o + __shfl_sync(0xffffffffu, prow, r) * DH + c * 64 + (q4 & 1) * 8 + (q4 & 2) * 2;
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {  // two 8-column groups: even lanes take the first, odd ones the second
+              const int e = 2 * b * 4 + k * 2;
+              uint32_t v[2][2] = {{x[e], x[e + 1]}, {x[e + 4], x[e + 5]}};
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                const uint32_t w = __shfl_xor_sync(0xffffffffu, lane & 1 ? v[0][i] : v[1][i], 1);
+                if (lane & 1) v[0][i] = w;
+                else v[1][i] = w;
+              }
+              if ((stored >> r) & 1) *reinterpret_cast<uint4*>(dst + b * 16) = make_uint4(v[0][0], v[0][1], v[1][0], v[1][1]);
+            }
+          }
+        }
+        o_done();
+        if (valid) {
+          *reinterpret_cast<float2*>(part_ml + prow * 2) = make_float2(mlog, l_run);
+          if (p.row_o != nullptr) p.row_parts[cls + orow] = flags & kWhole ? -1 : tl.parts;
+        }
       }
       release();
     }
@@ -831,18 +908,27 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 // ------------------------------------------------------------------------------------ joining parts
 // One row by one warp: part i (of `count`) has its maximum and sum at ml(i), its O at o(i); a lane
-// holds D / 32 columns. Lanes read up to 32 parts' maxima at once, then all O rows are in flight
-// four at a time.
+// holds D / 32 columns. Lanes read up to 32 parts' maxima at once, and O rows come four at a time, the
+// first four together with the maxima: the time is that of one or two reads.
 template <int DH, typename Ml, typename O>
 __device__ __forceinline__ void join_row(int count, Ml ml_of, O o_of, __nv_bfloat16* out, float* lse) {
   constexpr int CPL = DH / 32;
+  using Vec = typename std::conditional<CPL == 4, float4, float2>::type;
   const int lane = threadIdx.x & 31;
   float top = -INFINITY, total = 0.f, acc[CPL];
 #pragma unroll
   for (int k = 0; k < CPL; ++k) acc[k] = 0.f;
+#pragma unroll 1
   for (int i0 = 0; i0 < count; i0 += 32) {
+    const int m = min(32, count - i0);
+    Vec f[4];
+    auto fetch = [&](int i) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) f[u] = *reinterpret_cast<const Vec*>(o_of(i0 + min(i + u, m - 1)) + lane * CPL);
+    };
     float2 ml = make_float2(-INFINITY, 0.f);
-    if (i0 + lane < count) ml = *reinterpret_cast<const float2*>(ml_of(i0 + lane));
+    if (lane < m) ml = *reinterpret_cast<const float2*>(ml_of(i0 + lane));
+    fetch(0);
     float t = ml.x;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
@@ -856,26 +942,19 @@ __device__ __forceinline__ void join_row(int count, Ml ml_of, O o_of, __nv_bfloa
     top = t;
 #pragma unroll
     for (int k = 0; k < CPL; ++k) acc[k] *= old;
-    const int m = min(32, count - i0);
+#pragma unroll 1
     for (int i = 0; i < m; i += 4) {
-      float f[4][CPL];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const float* src = o_of(i0 + min(i + u, m - 1)) + lane * CPL;
-        if constexpr (CPL == 4) {
-          const float4 v = *reinterpret_cast<const float4*>(src);
-          f[u][0] = v.x, f[u][1] = v.y, f[u][2] = v.z, f[u][3] = v.w;
-        } else {
-          const float2 v = *reinterpret_cast<const float2*>(src);
-          f[u][0] = v.x, f[u][1] = v.y;
-        }
-      }
+      if (i) fetch(i);
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const float ws = __shfl_sync(0xffffffffu, w, (i + u) & 31);
         if (i + u < m) {
-#pragma unroll
-          for (int k = 0; k < CPL; ++k) acc[k] = fmaf(ws, f[u][k], acc[k]);
+          acc[0] = fmaf(ws, f[u].x, acc[0]);
+          acc[1] = fmaf(ws, f[u].y, acc[1]);
+          if constexpr (CPL == 4) {
+            acc[2] = fmaf(ws, f[u].z, acc[2]);
+            acc[3] = fmaf(ws, f[u].w, acc[3]);
+          }
         }
       }
     }
@@ -896,11 +975,13 @@ __device__ __forceinline__ long part_row(int parts, int i, int row) {
 __device__ __forceinline__ int part_count(int parts) { return (parts >> 16) - ((parts >> 8) & 255) + 1; }
 
 constexpr int kJoinThreads = 256;
-constexpr int kJoinSplit = 8;  // blocks per cut tile: 64 warps, row r by warp r mod 64
+constexpr int kJoinSplit = 16;  // blocks per cut tile: 128 warps, row r by warp r mod 128
 
 // The tile that block blockIdx.x began and did not finish.
 template <int DH>
 __global__ void __launch_bounds__(kJoinThreads) join_cut_tiles_kernel(PackedAttnParams p) {
+  wait_for_earlier_kernels();
+  let_later_kernels_start();
   const CutTile cut = p.cuts[blockIdx.x];
   if (cut.parts < 0) return;
   const int count = part_count(cut.parts);
@@ -920,6 +1001,8 @@ __global__ void __launch_bounds__(kJoinThreads) join_cut_tiles_kernel(PackedAttn
 // tokens from the request's first one, the prefix's tile from the batch's.
 template <int DH>
 __global__ void __launch_bounds__(kJoinThreads) join_rows_kernel(PackedAttnParams p) {
+  wait_for_earlier_kernels();
+  let_later_kernels_start();
   const long orow = (long)blockIdx.x * (kJoinThreads / 32) + (threadIdx.x >> 5);
   if (orow >= (long)p.N * p.H) return;
   const int tok = static_cast<int>(orow / p.H), head = static_cast<int>(orow - (long)tok * p.H);
@@ -957,14 +1040,34 @@ void launch(const CUtensorMap& q, const CUtensorMap& q1, const CUtensorMap& k, c
             const PackedAttnParams& p, cudaStream_t stream) {
   constexpr int smem = Cfg<DH>::SMEM + Cfg<DH>::TAIL;
   static_assert(smem <= 232448, "shared memory of a block");
+  static std::atomic<uint64_t> prepared{0};  // devices whose kernel may use that much
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 64 || !(prepared.load(std::memory_order_relaxed) >> dev & 1)) {
+    cudaFuncSetAttribute(packed_attention_kernel<DH>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (dev < 64) prepared.fetch_or(uint64_t(1) << dev, std::memory_order_relaxed);
+  }
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
   const int blocks = packed_attention_blocks();
-  cudaFuncSetAttribute(packed_attention_kernel<DH>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  packed_attention_kernel<DH><<<blocks, kThreads, smem, stream>>>(q, q1, k, v, p);
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchKernelEx(&cfg, packed_attention_kernel<DH>, q, q1, k, v, p);
+  cfg.blockDim = dim3(kJoinThreads);
+  cfg.dynamicSmemBytes = 0;
   if (p.row_o != nullptr) {
     const long per = kJoinThreads / 32;
-    join_rows_kernel<DH><<<static_cast<unsigned>(((long)p.N * p.H + per - 1) / per), kJoinThreads, 0, stream>>>(p);
+    cfg.gridDim = dim3(static_cast<unsigned>(((long)p.N * p.H + per - 1) / per));
+    cudaLaunchKernelEx(&cfg, join_rows_kernel<DH>, p);
   } else {
-    join_cut_tiles_kernel<DH><<<dim3(blocks, kJoinSplit), kJoinThreads, 0, stream>>>(p);
+    cfg.gridDim = dim3(blocks, kJoinSplit);
+    cudaLaunchKernelEx(&cfg, join_cut_tiles_kernel<DH>, p);
   }
 }
 
