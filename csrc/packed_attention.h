@@ -38,7 +38,7 @@ struct PackedAttnParams {
   CutTile* cuts;       // [blocks]
   float* row_o;        // with a prefix: [2, N, H, D] results of whole tiles (own keys, prefix),
   float* row_ml;       // [2, N, H, 2] their max and sum,
-  int* row_parts;      // [2, N, H] the row's parts (-1: whole tile)
+  int* row_parts;      // [2, N, H] the row's parts
   int* err;
 };
 

@@ -50,7 +50,10 @@ constexpr int kThreads = 384;      // three warpgroups: roles, softmax of half 0
 constexpr int kMaxBlocks = 256;    // blocks of a launch (one per SM)
 constexpr int kTiles = 4;          // published tiles in flight
 constexpr int kBlk = 128;          // keys per block = rows per page
-constexpr long kTileCost = 256;    // a tile's fixed cost, in keys (3.4 us beside 2.1 us for a key block of two halves)
+// a tile's fixed cost, in keys: 2.7 us beside 2.0 us for a key block of two halves; 3.6 us beside 1.3 us
+// for one of a tile of one half; a little above that, since a block that is late holds up all (96 answers:
+// 61 us against 63 at 192 / 384 and 68 at 192 / 256)
+constexpr long kTileCost = 256, kHalfTileCost = 512;
 constexpr long kLeastWork = 128;   // least stretch of a block: at least one block boundary lies in it,
                                    // so the blocks that share a tile's keys are consecutive
 
@@ -84,11 +87,13 @@ struct Tile {
 };
 
 // the parts of a cut tile: blocks ca .. cb, of which c0 (where the tile begins) uses its second slot
-__host__ __device__ __forceinline__ int pack_parts(int c0, int ca, int cb) { return c0 | ca << 8 | cb << 16; }
+__device__ __forceinline__ int pack_parts(int c0, int ca, int cb) { return c0 | ca << 8 | cb << 16; }
+constexpr int kWholeRow = 255 << 8;  // a row whose tile is whole (no parts: ca > cb)
 
 struct Request {
   int q0, q, past, kv, nt;
   bool shared;  // the prefix: every token of the batch, every key
+  bool half;    // the last tile has one half
   long base;    // cost of a tile before its own new tokens
   int slope;    // more keys per tile
 };
@@ -104,6 +109,7 @@ __device__ __forceinline__ Request make_request(const PackedAttnParams& p, int q
   r.shared = shared;
   const int tt2 = 2 * p.TT;
   r.nt = (r.q + tt2 - 1) / tt2;
+  r.half = r.nt * tt2 - r.q >= p.TT;
   r.base = kTileCost + (shared ? r.kv : max(r.past, 0));
   r.slope = shared ? 0 : tt2;
   return r;
@@ -117,17 +123,19 @@ __device__ __forceinline__ Request load_request(const PackedAttnParams& p, int i
 // cost of the first k tiles of one head
 __device__ __forceinline__ long tiles_cost(const Request& r, int k) {
   long c = k * r.base + (long)r.slope * k * (k + 1) / 2;
-  if (k == r.nt && r.slope) c -= (long)r.nt * r.slope - r.q;
+  if (k == r.nt) {
+    if (r.slope) c -= (long)r.nt * r.slope - r.q;
+    if (r.half) c += kHalfTileCost - kTileCost;
+  }
   return c;
 }
 // key blocks before point w of the line inside the tile [at, at + cost)
-__device__ __forceinline__ int cut_block(long w, long at, long cost, int nb) {
+__device__ __forceinline__ int cut_block(long w, long at, long cost, int nb, bool half) {
   if (w <= at) return 0;
   if (w >= at + cost) return nb;
-  const long s = (w - at - kTileCost + kBlk / 2) / kBlk;
+  const long s = (w - at - (half ? kHalfTileCost : kTileCost) + kBlk / 2) / kBlk;
   return static_cast<int>(min(max(s, 0L), static_cast<long>(nb)));
 }
-__device__ __forceinline__ long stretch(long W, int c, int n) { return W * c / n; }
 
 // Programmatic dependent launch: a kernel of this file starts while the one before it ends, and waits
 // here before it touches what that one (or any before it) wrote.
@@ -316,8 +324,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     for (int w = 0; w < kThreads / 32; ++w) W += scan[w];
   }
-  int n = 0;
-  long w0 = 0, w1 = 0, base = 0;
+  long L = 0, w0 = 0, w1 = 0, base = 0;  // stretches are L long, block c's begins at c * L
   for (int i0 = 0; i0 < E; i0 += kThreads) {
     if (i0 || E > kThreads) __syncthreads();
     const int i = i0 + tid;
@@ -343,9 +350,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (i0 == 0) {
       if (E <= kThreads) W = all;
-      n = static_cast<int>(min(max(W / kLeastWork, 1L), static_cast<long>(gridDim.x)));
-      w0 = stretch(W, me, n);
-      w1 = stretch(W, me + 1, n);
+      L = max((W + gridDim.x - 1) / static_cast<long>(gridDim.x), kLeastWork);
+      w0 = me * L;
+      w1 = min(w0 + L, W);
     }
     if (before + inc - v <= w0 && w0 < before + inc) {
       s_int[0] = i;
@@ -358,7 +365,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = s_int[1];
-  if (W == 0 || me >= n) {
+  if (w0 >= W) {
     if (tid == 0) p.cuts[me].parts = -1;
     if (warp == 1) tmem_dealloc(tmem, 512);
     return;
@@ -398,18 +405,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int vis0 = r.shared ? r.kv : min(max(r.past + t0 + min(ntok, p.TT), 0), r.kv);
         const int nb = (vis1 + kBlk - 1) / kBlk, nb0 = (vis0 + kBlk - 1) / kBlk;
         const bool owner = at >= w0;
-        const int jb = cut_block(w0, at, cost, nb), je = cut_block(w1, at, cost, nb);
+        const int jb = cut_block(w0, at, cost, nb, ntok <= p.TT), je = cut_block(w1, at, cost, nb, ntok <= p.TT);
         const bool whole = jb == 0 && je == nb;
         int parts = 0;
         if (!whole && (je > jb || owner)) {  // the blocks that share this tile: their stretches meet [at, at + cost)
-          const int c0 = static_cast<int>(((at + 1) * n + W - 1) / W) - 1;
-          const int c1 = static_cast<int>(((at + cost) * n + W - 1) / W) - 1;
+          const int c0 = static_cast<int>(at / L), c1 = static_cast<int>((at + cost - 1) / L);
           int ca = -1, cb = -1;
 #pragma unroll 1
           for (int c = c0; c <= c1; c += 32) {
             const int cl = c + lane;
-            const unsigned some = __ballot_sync(0xffffffffu, cl <= c1 && cut_block(stretch(W, cl + 1, n), at, cost, nb) >
-                                                                             cut_block(stretch(W, cl, n), at, cost, nb));
+            const unsigned some = __ballot_sync(0xffffffffu, cl <= c1 && cut_block((cl + 1) * L, at, cost, nb, ntok <= p.TT) >
+                                                                             cut_block(cl * L, at, cost, nb, ntok <= p.TT));
             if (some) {
               if (ca < 0) ca = c + __ffs(some) - 1;
               cb = c + 31 - __clz(some);
@@ -892,7 +898,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         o_done();
         if (valid) {
           *reinterpret_cast<float2*>(part_ml + prow * 2) = make_float2(mlog, l_run);
-          if (p.row_o != nullptr) p.row_parts[cls + orow] = flags & kWhole ? -1 : tl.parts;
+          // with the row's place inside the tile, where the slots have it
+          if (p.row_o != nullptr) p.row_parts[cls + orow] = flags & kWhole ? kWholeRow : tl.parts | ((alt ? 0 : hf * 128) + row) << 24;
         }
       }
       release();
@@ -908,9 +915,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 // ------------------------------------------------------------------------------------ joining parts
 // One row by one warp: part i (of `count`) has its maximum and sum at ml(i), its O at o(i); a lane
-// holds D / 32 columns. Lanes read up to 32 parts' maxima at once, and O rows come four at a time, the
-// first four together with the maxima: the time is that of one or two reads.
-template <int DH, typename Ml, typename O>
+// holds D / 32 columns. What it costs is reads after one another (about a microsecond each, for lines
+// that other SMs have just written): the lanes read up to 32 parts' maxima at once, and the O rows of
+// the first FLY parts are in flight together with them.
+template <int DH, int FLY, typename Ml, typename O>
 __device__ __forceinline__ void join_row(int count, Ml ml_of, O o_of, __nv_bfloat16* out, float* lse) {
   constexpr int CPL = DH / 32;
   using Vec = typename std::conditional<CPL == 4, float4, float2>::type;
@@ -921,10 +929,11 @@ __device__ __forceinline__ void join_row(int count, Ml ml_of, O o_of, __nv_bfloa
 #pragma unroll 1
   for (int i0 = 0; i0 < count; i0 += 32) {
     const int m = min(32, count - i0);
-    Vec f[4];
+    Vec f[FLY];
     auto fetch = [&](int i) {
 #pragma unroll
-      for (int u = 0; u < 4; ++u) f[u] = *reinterpret_cast<const Vec*>(o_of(i0 + min(i + u, m - 1)) + lane * CPL);
+      for (int u = 0; u < FLY; ++u)
+        if (i + u < m) f[u] = *reinterpret_cast<const Vec*>(o_of(i0 + i + u) + lane * CPL);
     };
     float2 ml = make_float2(-INFINITY, 0.f);
     if (lane < m) ml = *reinterpret_cast<const float2*>(ml_of(i0 + lane));
@@ -943,10 +952,10 @@ __device__ __forceinline__ void join_row(int count, Ml ml_of, O o_of, __nv_bfloa
 #pragma unroll
     for (int k = 0; k < CPL; ++k) acc[k] *= old;
 #pragma unroll 1
-    for (int i = 0; i < m; i += 4) {
+    for (int i = 0; i < m; i += FLY) {
       if (i) fetch(i);
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      for (int u = 0; u < FLY; ++u) {
         const float ws = __shfl_sync(0xffffffffu, w, (i + u) & 31);
         if (i + u < m) {
           acc[0] = fmaf(ws, f[u].x, acc[0]);
@@ -972,67 +981,84 @@ __device__ __forceinline__ long part_row(int parts, int i, int row) {
   const int c0 = parts & 255, c = ((parts >> 8) & 255) + i;
   return (long)(2 * c + (c == c0)) * kPaRows + row;
 }
-__device__ __forceinline__ int part_count(int parts) { return (parts >> 16) - ((parts >> 8) & 255) + 1; }
+__device__ __forceinline__ int part_count(int parts) { return ((parts >> 16) & 255) - ((parts >> 8) & 255) + 1; }
 
 constexpr int kJoinThreads = 256;
-constexpr int kJoinSplit = 16;  // blocks per cut tile: 128 warps, row r by warp r mod 128
+constexpr int kCutBlocksPerSm = 4;  // 64 registers: the first four parts stay in flight without spills
 
-// The tile that block blockIdx.x began and did not finish.
+// The rows of all cut tiles (at most one begins in each block of the attention kernel), shared out evenly.
 template <int DH>
-__global__ void __launch_bounds__(kJoinThreads) join_cut_tiles_kernel(PackedAttnParams p) {
+__global__ void __launch_bounds__(kJoinThreads, kCutBlocksPerSm) join_cut_tiles_kernel(PackedAttnParams p, int blocks) {
+  static_assert(kMaxBlocks <= kJoinThreads, "one thread per noted tile");
+  __shared__ CutTile s_cut[kMaxBlocks];
+  __shared__ int s_end[kMaxBlocks];  // rows up to and with this tile's
+  __shared__ int s_warp[kMaxBlocks / 32];
   wait_for_earlier_kernels();
   let_later_kernels_start();
-  const CutTile cut = p.cuts[blockIdx.x];
-  if (cut.parts < 0) return;
-  const int count = part_count(cut.parts);
-  for (int r = (threadIdx.x >> 5) * kJoinSplit + blockIdx.y; r < kPaRows; r += kJoinSplit * (kJoinThreads / 32)) {
-    const int hr = r & 127, rtok = hr / p.G, tk = (r >> 7) * p.TT + rtok;
-    if (rtok >= p.TT || tk >= cut.ntok) continue;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int rows = 0;
+  if (tid < kMaxBlocks) {
+    CutTile cut;
+    cut.parts = -1;
+    if (tid < blocks) cut = p.cuts[tid];
+    s_cut[tid] = cut;
+    rows = cut.parts >= 0 ? cut.ntok * p.G : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, rows, o);
+      if (lane >= o) rows += up;
+    }
+    if (lane == 31) s_warp[warp] = rows;
+  }
+  __syncthreads();
+  if (tid < kMaxBlocks) {
+    for (int w = 0; w < warp; ++w) rows += s_warp[w];
+    s_end[tid] = rows;
+  }
+  __syncthreads();
+  const int all = s_end[kMaxBlocks - 1];
+  for (int u = warp * gridDim.x + blockIdx.x; u < all; u += gridDim.x * (kJoinThreads / 32)) {
+    int lo = 0, hi = kMaxBlocks - 1;  // the first tile that ends after row u
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (s_end[mid] > u) hi = mid;
+      else lo = mid + 1;
+    }
+    const CutTile cut = s_cut[lo];
+    const int r = u - (lo ? s_end[lo - 1] : 0), tk = r / p.G, g = r - tk * p.G;
+    const int row = (tk >= p.TT ? 128 + (tk - p.TT) * p.G : tk * p.G) + g;
     const long tok = cut.tok0 + tk;
-    const int head = cut.hv * p.G + hr - rtok * p.G;
-    join_row<DH>(count, [&](int i) { return p.slot_ml + part_row(cut.parts, i, r) * 2; },
-                 [&](int i) { return p.slots + part_row(cut.parts, i, r) * DH; }, p.o + tok * p.ldo + (long)head * DH,
+    const int head = cut.hv * p.G + g;
+    join_row<DH, 4>(part_count(cut.parts), [&](int i) { return p.slot_ml + part_row(cut.parts, i, row) * 2; },
+                 [&](int i) { return p.slots + part_row(cut.parts, i, row) * DH; }, p.o + tok * p.ldo + (long)head * DH,
                  p.lse != nullptr ? p.lse + tok * p.H + head : nullptr);
   }
 }
 
 // Every row of a batch that shares a prefix: its own parts and the prefix's. A whole tile's part lies
-// in the row buffers, a cut one's in the slots, at the row's place inside its tile: the own tile counts
-// tokens from the request's first one, the prefix's tile from the batch's.
+// in the row buffers, a cut one's in the slots, at the row's place inside its tile.
 template <int DH>
 __global__ void __launch_bounds__(kJoinThreads) join_rows_kernel(PackedAttnParams p) {
   wait_for_earlier_kernels();
   let_later_kernels_start();
-  const long orow = (long)blockIdx.x * (kJoinThreads / 32) + (threadIdx.x >> 5);
-  if (orow >= (long)p.N * p.H) return;
+  const long cls = (long)p.N * p.H, orow = (long)blockIdx.x * (kJoinThreads / 32) + (threadIdx.x >> 5);
+  if (orow >= cls) return;
+  const int own = p.row_parts[orow], pre = p.row_parts[cls + orow];
   const int tok = static_cast<int>(orow / p.H), head = static_cast<int>(orow - (long)tok * p.H);
   if (tok >= p.q_start[p.B]) return;
-  const long cls = (long)p.N * p.H;
-  const int own = p.row_parts[orow], pre = p.row_parts[cls + orow];
-  const int hr = head % p.G, tt2 = 2 * p.TT;
-  auto place = [&](int t) { return (t % tt2) / p.TT * 128 + (t % p.TT) * p.G + hr; };
-  int own_row = 0;
-  if (own >= 0) {  // the request's first token
-    int lo = 0, hi = p.B;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (p.q_start[mid] <= tok) lo = mid;
-      else hi = mid;
-    }
-    own_row = place(tok - p.q_start[lo]);
-  }
-  const int pre_row = place(tok);
-  const int n_own = own < 0 ? 1 : part_count(own), n_pre = pre < 0 ? 1 : part_count(pre);
-  join_row<DH>(n_own + n_pre,
+  auto whole = [](int parts) { return (parts & 0xffffff) == kWholeRow; };
+  const int n_own = whole(own) ? 1 : part_count(own), n_pre = whole(pre) ? 1 : part_count(pre);
+  const int own_row = static_cast<unsigned>(own) >> 24, pre_row = static_cast<unsigned>(pre) >> 24;
+  join_row<DH, 8>(n_own + n_pre,
                [&](int i) -> const float* {
-                 if (i < n_own) return own < 0 ? p.row_ml + orow * 2 : p.slot_ml + part_row(own, i, own_row) * 2;
-                 return pre < 0 ? p.row_ml + (cls + orow) * 2 : p.slot_ml + part_row(pre, i - n_own, pre_row) * 2;
+                 if (i < n_own) return whole(own) ? p.row_ml + orow * 2 : p.slot_ml + part_row(own, i, own_row) * 2;
+                 return whole(pre) ? p.row_ml + (cls + orow) * 2 : p.slot_ml + part_row(pre, i - n_own, pre_row) * 2;
                },
                [&](int i) -> const float* {
-                 if (i < n_own) return own < 0 ? p.row_o + orow * DH : p.slots + part_row(own, i, own_row) * DH;
-                 return pre < 0 ? p.row_o + (cls + orow) * DH : p.slots + part_row(pre, i - n_own, pre_row) * DH;
+                 if (i < n_own) return whole(own) ? p.row_o + orow * DH : p.slots + part_row(own, i, own_row) * DH;
+                 return whole(pre) ? p.row_o + (cls + orow) * DH : p.slots + part_row(pre, i - n_own, pre_row) * DH;
                },
-               p.o + tok * p.ldo + (long)head * DH, p.lse != nullptr ? p.lse + orow : nullptr);
+               p.o + (long)tok * p.ldo + (long)head * DH, p.lse != nullptr ? p.lse + orow : nullptr);
 }
 
 template <int DH>
@@ -1066,8 +1092,8 @@ void launch(const CUtensorMap& q, const CUtensorMap& q1, const CUtensorMap& k, c
     cfg.gridDim = dim3(static_cast<unsigned>(((long)p.N * p.H + per - 1) / per));
     cudaLaunchKernelEx(&cfg, join_rows_kernel<DH>, p);
   } else {
-    cfg.gridDim = dim3(blocks, kJoinSplit);
-    cudaLaunchKernelEx(&cfg, join_cut_tiles_kernel<DH>, p);
+    cfg.gridDim = dim3(kCutBlocksPerSm * blocks);
+    cudaLaunchKernelEx(&cfg, join_cut_tiles_kernel<DH>, p, blocks);
   }
 }
 
