@@ -267,8 +267,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   float2* s_ml = reinterpret_cast<float2*>(bars + 44);    // [128]
   Tile* tiles = reinterpret_cast<Tile*>(s_ml + 128);
   long* scan = reinterpret_cast<long*>(tiles + kTiles);   // the warps' sums, the begin's offset
-  int* s_int = reinterpret_cast<int*>(scan + kThreads / 32 + 1);  // begin's entry, TMEM base
-  static_assert(sizeof(Tile) * kTiles % 8 == 0 && 44 * 8 + 1024 + sizeof(Tile) * kTiles + 8 * (kThreads / 32 + 1) + 8 <= 2048,
+  int* s_int = reinterpret_cast<int*>(scan + kThreads / 32 + 1);  // begin's entry, TMEM base, the entry's tokens and keys
+  static_assert(sizeof(Tile) * kTiles % 8 == 0 && 44 * 8 + 1024 + sizeof(Tile) * kTiles + 8 * (kThreads / 32 + 1) + 24 <= 2048,
                 "the tail holds what lies in it");
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -329,8 +329,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (i0 || E > kThreads) __syncthreads();
     const int i = i0 + tid;
     long v = 0;
+    Request r{};
     if (i < E) {
-      const Request r = load_request(p, i);
+      r = load_request(p, i);
       v = p.Hv * tiles_cost(r, r.nt);
     }
     long inc = v;
@@ -356,6 +357,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (before + inc - v <= w0 && w0 < before + inc) {
       s_int[0] = i;
+      s_int[2] = r.q0;
+      s_int[3] = r.q0 + r.q;
+      s_int[4] = r.kv;
       scan[kThreads / 32] = w0 - (before + inc - v);
     }
     base += all;
@@ -379,7 +383,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // ---------------------------------------------------------------------------- work list + TMA
       bool ok = true;
       int e = s_int[0];
-      Request r = load_request(p, e);
+      Request r = make_request(p, s_int[2], s_int[3], s_int[4], p.shared_len > 0 && e == 0);
       const long head_cost = tiles_cost(r, r.nt);
       const long off = scan[kThreads / 32];
       int hv = static_cast<int>(off / head_cost), t = 0;
@@ -407,6 +411,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool owner = at >= w0;
         const int jb = cut_block(w0, at, cost, nb, ntok <= p.TT), je = cut_block(w1, at, cost, nb, ntok <= p.TT);
         const bool whole = jb == 0 && je == nb;
+        const int kvh = hv / p.ng, b = p.shared_len > 0 ? e - 1 : e;
+        const int* pages = r.shared ? p.prefix : p.table != nullptr ? p.table + b * p.ld_table : nullptr;
+        const int npages = r.shared ? p.prefix_pages : p.W;
+        auto fetch_pages = [&](int j) { return jb + j + lane < npages && j + lane < je - jb ? pages[jb + j + lane] : -1; };
+        int pg = pages != nullptr ? fetch_pages(0) : 0;  // on its way while the parts are worked out
         int parts = 0;
         if (!whole && (je > jb || owner)) {  // the blocks that share this tile: their stretches meet [at, at + cost)
           const int c0 = static_cast<int>(at / L), c1 = static_cast<int>((at + cost - 1) / L);
@@ -449,16 +458,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_arrive(smem_addr(&t_full[np % kTiles]));
           }
           ++np;
-          const int kvh = hv / p.ng, b = p.shared_len > 0 ? e - 1 : e;
-          const int* pages = r.shared ? p.prefix : p.table != nullptr ? p.table + b * p.ld_table : nullptr;
-          const int npages = r.shared ? p.prefix_pages : p.W;
-          int pg = 0;
           for (int j = 0; ok && j < je - jb; ++j) {
             const int blk = jb + j;
             int row;
             if (pages != nullptr) {
               if ((j & 31) == 0) {
-                pg = blk + lane < npages && j + lane < je - jb ? pages[blk + lane] : -1;
+                if (j) pg = fetch_pages(j);
                 if (pg < 0 || pg >= p.pages) pg = p.pages;  // no page: past the pool, where TMA fills zeros
               }
               row = __shfl_sync(0xffffffffu, pg, j & 31) * kBlk;
@@ -848,6 +853,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           load_o(h, c, x);
 #pragma unroll
           for (int k = 0; k < 2; ++k) {  // rows lane / 4 and lane / 4 + 8 of the 16
+            if (!((stored >> (16 * h + 8 * k)) & 0xFFu)) continue;
             const int r = 16 * h + 8 * k + lane / 4;
             const float w = __shfl_sync(0xffffffffu, inv, r);
             bf16* dst = p.o + __shfl_sync(0xffffffffu, at, r) + c * 64 + q4 * 8;
@@ -879,6 +885,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           load_o(h, c, x);
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
+            if (!((stored >> (16 * h + 8 * k)) & 0xFFu)) continue;
             const int r = 16 * h + 8 * k + lane / 4;
             float* dst = part_o + __shfl_sync(0xffffffffu, prow, r) * DH + c * 64 + (q4 & 1) * 8 + (q4 & 2) * 2;
 #pragma unroll
