@@ -34,6 +34,17 @@
 // Keys past a request's end in its last page may hold anything: their scores are replaced, and
 // their V rows are zeroed in shared memory, since 0 * NaN would reach the accumulators.
 // All waits are bounded; a wait that runs out sets the error word and every role leaves.
+//
+// What bounds it. Long prompts (four of 3010 to 5001 tokens, 28 heads of 128 over 4, 487 GFLOP): 480 to 510
+// us, about 1 PFLOP/s. A key block of a half is 3700 clocks from one S to the next: 2000 of softmax
+// (exponentials 1280, at the special-function unit's rate; maxima 390; TMEM reads and writes 310), 1024
+// of products, the rest hand-offs; the tensor core is busy a little over half of the time. Tried and not
+// kept: a quarter or half of the exponentials on the fp32 pipe (equal / 10 % slower), 16 softmax warps
+// with a row over four lanes (equal on prompts, 1 us slower on small calls). Answers (96 of 60 to 6000
+// keys, 237 MB): 60 us, 3.9 TB/s; each SM's stretches hold 1 to 10 tiles, and a tile's turnaround (3.6 us:
+// last product, output, next tile's first scores) is only partly covered by the loads ahead of it. Small
+// calls (10 us): 2 us of work line, 1.5 us of loads, 1.3 us for the first softmax, 1 us of output, and the
+// joining kernel.
 #include "packed_attention.h"
 
 #include <atomic>
@@ -142,16 +153,14 @@ __device__ __forceinline__ int cut_block(long w, long at, long cost, int nb, boo
 __device__ __forceinline__ void wait_for_earlier_kernels() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_later_kernels_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
-// Bounded wait of a whole warp. It polls without reading a clock: the waits lie on the chain of
-// S, softmax, P V, and a wait that reads the global timer as soon as its first poll fails (as
-// mbar_wait does) took 2.4 us for a key block where 1.1 us of products are done. 2^22 polls, each of
-// which the hardware may suspend for a while, are tenths of a second at the least; tiles take less than
-// a millisecond.
+// Bounded wait of a whole warp. It counts polls and reads no clock: the waits lie on the chain of S,
+// softmax and P V, and the clock's code beside them cost 2 to 4 %. The hardware suspends a poll that
+// fails for 1.3 us, so 2^20 of them are 1.4 s; tiles take less than a few milliseconds.
 __device__ __forceinline__ bool poll(uint32_t bar, uint32_t parity, int* err, int code) {
 #pragma unroll 1
-  for (int i = 0; i < (1 << 22); ++i) {
+  for (int i = 0; i < (1 << 20); ++i) {
     if (mbar_try_wait(bar, parity)) return true;
-    if ((i & 1023) == 1023 && error_raised(err)) return false;
+    if ((i & 255) == 255 && error_raised(err)) return false;
   }
   record_error(err, code);
   return false;

@@ -8,7 +8,8 @@
 //   token n = q_start[b] + i:  req = b, pos = past[b] + i, row = page(pos / 128) * 128 + pos % 128
 // and free_next = (first free index after this step, pages that could not be given).
 //
-// Nothing but latency bounds it (12 bytes a token out: 224k tokens are 2.7 MB), so it is ONE launch:
+// Nothing but latency bounds it (12 bytes a token out: the 224k tokens of 2048 requests are 2.7 MB and take
+// 6.6 us, one request's token 2.9 us), so it is ONE launch:
 // every block scans all the requests itself, 1024 at a time in shared memory, which costs less than
 // a second launch or a look-back between blocks would; block k then owns an equal share of the
 // tokens (request found by a binary search in shared memory) and every gridDim-th request's new
