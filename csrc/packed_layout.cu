@@ -171,6 +171,8 @@ void packed_layout_op(const at::Tensor& q_len, const at::Tensor& past, at::Tenso
     APPCORR_CHECK(t->device() == q_len.device(), "packed_layout: tensors on different devices");
   APPCORR_CHECK(free_next.data_ptr() != free_start.data_ptr(),
               "packed_layout: free_next must not be free_start (every block reads it)");
+  APPCORR_CHECK(B == 0 || (kv_len.data_ptr() != past.data_ptr() && kv_len.data_ptr() != q_len.data_ptr()),
+                "packed_layout: kv_len must not be past or q_len (every block reads them)");
   c10::cuda::CUDAGuard guard(q_len.device());
   LayoutParams p{q_len.data_ptr<int>(), past.data_ptr<int>(), table.data_ptr<int>(), table.stride(0),
                  free_pages.data_ptr<int>(), free_start.data_ptr<int>(), q_start.data_ptr<int>(), kv_len.data_ptr<int>(),

@@ -139,7 +139,8 @@ def test_layout_refusals():
 
     call()
     start = e(2)
-    for kw in (dict(past=e(2)), dict(table=e(2, 4)), dict(q_start=e(3)), dict(req=e(4)), dict(free_next=e(1)), dict(kv_len=e(3).long()),
+    lens = e(3)
+    for kw in (dict(past=lens, kv_len=lens), dict(q_len=lens, kv_len=lens), dict(past=e(2)), dict(table=e(2, 4)), dict(q_start=e(3)), dict(req=e(4)), dict(free_next=e(1)), dict(kv_len=e(3).long()),
                dict(rows=e(5).cpu()), dict(table=e(4, 3).t()), dict(free_start=start[:1], free_next=start)):
         with pytest.raises(RuntimeError):
             call(**kw)
