@@ -21,7 +21,7 @@
 // completed, so a softmax warp that has S_j may rescale O, and S_{j+1} may overwrite P_j once PV_j
 // was issued.
 //
-// Work line. All tiles' costs (visible keys plus kTileCost for a tile's own start and end) are laid
+// Work line. All tiles' costs (their visible keys, and a tile's own start and end) are laid
 // on one line, the shared prefix's tiles first, then by request, key head and tile; every block
 // takes an equal stretch of it, so a stretch may begin and end inside a tile, on a key block. That
 // balances prompts of any mix of lengths and splits few long rows over all SMs by the same rule,
@@ -61,10 +61,9 @@ constexpr int kThreads = 384;      // three warpgroups: roles, softmax of half 0
 constexpr int kMaxBlocks = 256;    // blocks of a launch (one per SM)
 constexpr int kTiles = 4;          // published tiles in flight
 constexpr int kBlk = 128;          // keys per block = rows per page
-// a tile's fixed cost, in keys: 2.7 us beside 2.0 us for a key block of two halves; 3.6 us beside 1.3 us
-// for one of a tile of one half; a little above that, since a block that is late holds up all (96 answers:
-// 61 us against 63 at 192 / 384 and 68 at 192 / 256)
-constexpr long kTileCost = 256, kHalfTileCost = 512;
+// costs on the work line; a key block of two halves (2.0 us) is 128, one of a single half (1.3 us) 80, and a
+// tile's own start and end (2.7 us; 3.6 us for a single half; more where 256 rows leave fp32 parts)
+constexpr long kTileCost = 256, kTilePartsCost = 448, kHalfTileCost = 320, kHalfBlockCost = 80;
 constexpr long kLeastWork = 128;   // least stretch of a block: at least one block boundary lies in it,
                                    // so the blocks that share a tile's keys are consecutive
 
@@ -105,7 +104,8 @@ struct Request {
   int q0, q, past, kv, nt;
   bool shared;  // the prefix: every token of the batch, every key
   bool half;    // the last tile has one half
-  long base;    // cost of a tile before its own new tokens
+  long fixed;   // cost of a tile of two halves without its keys
+  long base;    // ... and before its own new tokens
   int slope;    // more keys per tile
 };
 
@@ -121,7 +121,8 @@ __device__ __forceinline__ Request make_request(const PackedAttnParams& p, int q
   const int tt2 = 2 * p.TT;
   r.nt = (r.q + tt2 - 1) / tt2;
   r.half = r.nt * tt2 - r.q >= p.TT;
-  r.base = kTileCost + (shared ? r.kv : max(r.past, 0));
+  r.fixed = p.row_o != nullptr ? kTilePartsCost : kTileCost;
+  r.base = r.fixed + (shared ? r.kv : max(r.past, 0));
   r.slope = shared ? 0 : tt2;
   return r;
 }
@@ -136,15 +137,18 @@ __device__ __forceinline__ long tiles_cost(const Request& r, int k) {
   long c = k * r.base + (long)r.slope * k * (k + 1) / 2;
   if (k == r.nt) {
     if (r.slope) c -= (long)r.nt * r.slope - r.q;
-    if (r.half) c += kHalfTileCost - kTileCost;
+    if (r.half) {  // the last tile's keys at the other price
+      const long keys = r.base - r.fixed + (r.slope ? r.q : 0);
+      c += kHalfTileCost + keys * kHalfBlockCost / kBlk - r.fixed - keys;
+    }
   }
   return c;
 }
 // key blocks before point w of the line inside the tile [at, at + cost)
-__device__ __forceinline__ int cut_block(long w, long at, long cost, int nb, bool half) {
+__device__ __forceinline__ int cut_block(long w, long at, long cost, int nb, bool half, long fixed) {
   if (w <= at) return 0;
   if (w >= at + cost) return nb;
-  const long s = (w - at - (half ? kHalfTileCost : kTileCost) + kBlk / 2) / kBlk;
+  const long s = half ? (w - at - kHalfTileCost + kHalfBlockCost / 2) / kHalfBlockCost : (w - at - fixed + kBlk / 2) / kBlk;
   return static_cast<int>(min(max(s, 0L), static_cast<long>(nb)));
 }
 
@@ -418,7 +422,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int vis0 = r.shared ? r.kv : min(max(r.past + t0 + min(ntok, p.TT), 0), r.kv);
         const int nb = (vis1 + kBlk - 1) / kBlk, nb0 = (vis0 + kBlk - 1) / kBlk;
         const bool owner = at >= w0;
-        const int jb = cut_block(w0, at, cost, nb, ntok <= p.TT), je = cut_block(w1, at, cost, nb, ntok <= p.TT);
+        const int jb = cut_block(w0, at, cost, nb, ntok <= p.TT, r.fixed), je = cut_block(w1, at, cost, nb, ntok <= p.TT, r.fixed);
         const bool whole = jb == 0 && je == nb;
         const int kvh = hv / p.ng, b = p.shared_len > 0 ? e - 1 : e;
         const int* pages = r.shared ? p.prefix : p.table != nullptr ? p.table + b * p.ld_table : nullptr;
@@ -432,8 +436,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
           for (int c = c0; c <= c1; c += 32) {
             const int cl = c + lane;
-            const unsigned some = __ballot_sync(0xffffffffu, cl <= c1 && cut_block((cl + 1) * L, at, cost, nb, ntok <= p.TT) >
-                                                                             cut_block(cl * L, at, cost, nb, ntok <= p.TT));
+            const unsigned some = __ballot_sync(0xffffffffu, cl <= c1 && cut_block((cl + 1) * L, at, cost, nb, ntok <= p.TT, r.fixed) >
+                                                                             cut_block(cl * L, at, cost, nb, ntok <= p.TT, r.fixed));
             if (some) {
               if (ca < 0) ca = c + __ffs(some) - 1;
               cb = c + 31 - __clz(some);
