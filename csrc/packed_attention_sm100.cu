@@ -41,7 +41,7 @@
 // of products, the rest hand-offs; the tensor core is busy a little over half of the time. Tried and not
 // kept: a quarter or half of the exponentials on the fp32 pipe (equal / 10 % slower), 16 softmax warps
 // with a row over four lanes (equal on prompts, 1 us slower on small calls). Answers (96 of 60 to 6000
-// keys, 237 MB): 60 us, 3.9 TB/s; each SM's stretches hold 1 to 10 tiles, and a tile's turnaround (3.6 us:
+// keys, 237 MB): 60 to 62 us, 3.9 TB/s; each SM's stretches hold 1 to 10 tiles, and a tile's turnaround (3.6 us:
 // last product, output, next tile's first scores) is only partly covered by the loads ahead of it. Small
 // calls (10 us): 2 us of work line, 1.5 us of loads, 1.3 us for the first softmax, 1 us of output, and the
 // joining kernel.
@@ -62,7 +62,9 @@ constexpr int kMaxBlocks = 256;    // blocks of a launch (one per SM)
 constexpr int kTiles = 4;          // published tiles in flight
 constexpr int kBlk = 128;          // keys per block = rows per page
 // costs on the work line; a key block of two halves (2.0 us) is 128, one of a single half (1.3 us) 80, and a
-// tile's own start and end (2.7 us; 3.6 us for a single half; more where 256 rows leave fp32 parts)
+// tile's own start and end (2.7 us; 3.6 us for a single half; more where 256 rows leave fp32 parts). With one
+// price for all key blocks 128 answers after a shared prefix took 71 us for 64, 144 answers of 8 key heads 110
+// for 87.
 constexpr long kTileCost = 256, kTilePartsCost = 448, kHalfTileCost = 320, kHalfBlockCost = 80;
 constexpr long kLeastWork = 128;   // least stretch of a block: at least one block boundary lies in it,
                                    // so the blocks that share a tile's keys are consecutive

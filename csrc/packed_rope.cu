@@ -11,7 +11,7 @@
 // formed in one fp32 product would be off by 1e-3 rad at position 30000.
 //
 // Bound: HBM, every projected value read once and written once (20011 tokens of 48 heads x 64: 246 MB in
-// 46 us = 5.3 TB/s, 0.83 of a plain copy; 1424 tokens of 36 x 128: 26 MB in 5.8 us; 61 of them: 2.8 us).
+// 46 us = 5.3 TB/s, 0.83 of a plain copy; 1424 tokens of 36 x 128: 26 MB in 5.5 us; 61 of them: 2.9 us).
 // A lane holds 8 values of a head's first half and the 8 they are paired with, so both loads and
 // stores are 16 bytes and the rotation needs no exchange; a head is D / 16 lanes (the norm is 3 or
 // 2 shuffles) and a warp walks its token's heads 32 / (D / 16) at a time with the next ones' loads
