@@ -74,9 +74,10 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch
     token t of request b sees the first kv_len[b] - q_len[b] + t + 1 of its keys.
 
     Keys are cache pages (table [>= B, W] into pools k / v of whole pages) or, with k_start [B], the
-    kv_len[b] packed rows of k / v from k_start[b]. Rows past q_start[B] are not touched; a token
-    that sees no key gets zeros (lse -inf). Cached rows past kv_len may hold anything. lse: fp32
-    [N, heads] natural log-sum-exp of the scaled scores. scale: head_dim ** -0.5 by default."""
+    kv_len[b] packed rows of k / v from k_start[b]. Rows before q_start[0] or past q_start[B] are not
+    touched (a call may take some of the batch's requests: slices of q_start, kv_len and table); a token
+    that sees no key gets zeros (lse -inf). Cached rows past kv_len may hold anything. lse: fp32 [N, heads]
+    natural log-sum-exp of the scaled scores. scale: head_dim ** -0.5 by default."""
     _count(2)
     lib().packed_attention(q, k, v, o, q_start, kv_len, heads, kv_heads, head_dim,
                            head_dim ** -0.5 if scale is None else scale, table, k_start, None, 0, lse, _err(q))
@@ -88,8 +89,8 @@ def shared_prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o
                             heads: int, kv_heads: int, head_dim: int, scale: Optional[float] = None,
                             lse: Optional[torch.Tensor] = None) -> torch.Tensor:
     """packed_attention for a batch whose requests continue one shared prefix: its prefix_len keys
-    (pages prefix_table [>= ceil(prefix_len / 128)] of the same pools) are visible to every token, in
-    front of the request's own kv_len[b] keys, which are paged through `table` and causal as there.
+    (pages prefix_table [>= ceil(prefix_len / 128)] of the same pools) are visible to every token of the
+    call's requests, in front of the request's own kv_len[b] keys, which are paged through `table` and causal as there.
     kv_len counts a request's own keys only and may be zero."""
     _count(2)
     lib().packed_attention(q, k, v, o, q_start, kv_len, heads, kv_heads, head_dim,

@@ -104,7 +104,7 @@ constexpr int kWholeRow = 255 << 8;  // a row whose tile is whole (no parts: ca 
 
 struct Request {
   int q0, q, past, kv, nt;
-  bool shared;  // the prefix: every token of the batch, every key
+  bool shared;  // the prefix: every token of the requests, every key
   bool half;    // the last tile has one half
   long fixed;   // cost of a tile of two halves without its keys
   long base;    // ... and before its own new tokens
@@ -131,7 +131,7 @@ __device__ __forceinline__ Request make_request(const PackedAttnParams& p, int q
 // entry i of the work line: the prefix (if there is one), then the requests
 __device__ __forceinline__ Request load_request(const PackedAttnParams& p, int i) {
   const int b = p.shared_len > 0 ? i - 1 : i;
-  if (b < 0) return make_request(p, 0, p.q_start[p.B], p.shared_len, true);
+  if (b < 0) return make_request(p, p.q_start[0], p.q_start[p.B], p.shared_len, true);
   return make_request(p, p.q_start[b], p.q_start[b + 1], p.kv_len[b], false);
 }
 // cost of the first k tiles of one head
@@ -1067,7 +1067,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_rows_kernel(PackedAttnParam
   if (orow >= cls) return;
   const int own = p.row_parts[orow], pre = p.row_parts[cls + orow];
   const int tok = static_cast<int>(orow / p.H), head = static_cast<int>(orow - (long)tok * p.H);
-  if (tok >= p.q_start[p.B]) return;
+  if (tok < p.q_start[0] || tok >= p.q_start[p.B]) return;  // no request's row
   auto whole = [](int parts) { return (parts & 0xffffff) == kWholeRow; };
   const int n_own = whole(own) ? 1 : part_count(own), n_pre = whole(pre) ? 1 : part_count(pre);
   const int own_row = static_cast<unsigned>(own) >> 24, pre_row = static_cast<unsigned>(pre) >> 24;

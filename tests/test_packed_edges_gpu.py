@@ -1,0 +1,55 @@
+"""Packed-batch operators (ops/packed.py) at the edges of their contracts: slices of a batch, arguments
+that are refused, values on the device that no request should bring. Tolerances are those of
+test_packed_gpu.py, whose cases and 64-bit statements are used here."""
+import pytest
+import torch
+
+from test_packed_gpu import DEV, Case, _done, _i, _packed
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------------------------ slices of a batch
+def _two_groups(prefixes, paged=True):
+    """Two groups of requests, each with a pool and a prefix of its own, whose tokens share one batch."""
+    a = Case([3, 1, 40], [9, 300, 40], 4, 2, 64, prefix=prefixes[0], seed=61, paged=paged)
+    b = Case([1, 70, 5], [700, 90, 5], 4, 2, 64, prefix=prefixes[1], seed=62, paged=paged)
+    n = a.N
+    q = torch.cat([a.q, b.q])
+    o = torch.full_like(q, 7.0)
+    lse = torch.full((q.shape[0], 4), 7.0, device=DEV)
+    start = _i(a.start + [n + s for s in b.start[1:]])
+    for c, rows, at in ((a, slice(0, n), slice(0, 4)), (b, slice(n, None), slice(3, 7))):
+        c.o, c.lse, c.at = o[rows], lse[rows], start[at]
+
+    def run(c):
+        P, kw = _packed(), dict(q_start=c.at, kv_len=_i(c.own), heads=4, kv_heads=2, head_dim=64, table=c.table, lse=lse)
+        if c.prefix:
+            P.shared_prefix_attention(q, c.k, c.v, o, prefix_table=c.prefix_table, prefix_len=c.prefix, **kw)
+        else:
+            P.packed_attention(q, c.k, c.v, o, k_start=c.k_start, **kw)
+        _done()
+
+    return a, b, run
+
+
+@pytest.mark.parametrize("prefixes", [(200, 1000), (1000, 130), (0, 500), (500, 0), (0, 0)])
+def test_groups_of_one_batch(prefixes):
+    """Each call leaves the other group's rows alone, whichever comes first."""
+    for order in (0, 1):
+        a, b, run = _two_groups(prefixes)
+        first, second = (b, a) if order else (a, b)
+        run(first)
+        assert bool((second.o == 7).all()) and bool((second.lse == 7).all())
+        kept, kept_lse = first.o.clone(), first.lse.clone()
+        run(second)
+        assert torch.equal(first.o, kept) and torch.equal(first.lse, kept_lse)
+        for c in (a, b):
+            c.check()
+
+
+def test_slice_without_requests():
+    a, b, run = _two_groups((200, 300))
+    b.at, b.own = b.at[:1], []
+    run(b)
+    assert bool((a.o == 7).all()) and bool((b.o == 7).all())
