@@ -33,7 +33,7 @@
 //
 // Keys past a request's end in its last page may hold anything: their scores are replaced, and
 // their V rows are zeroed in shared memory, since 0 * NaN would reach the accumulators.
-// All waits are bounded; a wait that runs out sets the error word and every role leaves.
+// All waits are bounded; a wait that runs out sets the error word, every role leaves and no row is joined.
 //
 // What bounds it. Long prompts (four of 3010 to 5001 tokens, 28 heads of 128 over 4, 487 GFLOP): 480 to 510
 // us, about 1 PFLOP/s. A key block of a half is 3700 clocks from one S to the next: 2000 of softmax
@@ -999,8 +999,10 @@ __device__ __forceinline__ void join_row(int count, Ml ml_of, O o_of, __nv_bfloa
   if (lse != nullptr && lane == 0) *lse = (top + log2f(total)) * 0.69314718055994531f;
 }
 
-__device__ __forceinline__ long part_row(int parts, int i, int row) {
-  const int c0 = parts & 255, c = ((parts >> 8) & 255) + i;
+// place of part i: inside the slots whatever the part numbers are (after a wait that ran out they may be
+// what the workspace held before)
+__device__ __forceinline__ long part_row(int parts, int i, int row, int blocks) {
+  const int c0 = parts & 255, c = min(((parts >> 8) & 255) + i, blocks - 1);
   return (long)(2 * c + (c == c0)) * kPaRows + row;
 }
 __device__ __forceinline__ int part_count(int parts) { return ((parts >> 16) & 255) - ((parts >> 8) & 255) + 1; }
@@ -1022,7 +1024,9 @@ __global__ void __launch_bounds__(kJoinThreads, kCutBlocksPerSm) join_cut_tiles_
   if (tid < kMaxBlocks) {
     CutTile cut;
     cut.parts = -1;
+    const bool failed = error_raised(p.err);  // the parts are not there: no row is joined
     if (tid < blocks) cut = p.cuts[tid];
+    if (failed) cut.parts = -1;
     s_cut[tid] = cut;
     rows = cut.parts >= 0 ? cut.ntok * p.G : 0;
 #pragma unroll
@@ -1051,8 +1055,8 @@ __global__ void __launch_bounds__(kJoinThreads, kCutBlocksPerSm) join_cut_tiles_
     const int row = (tk >= p.TT ? 128 + (tk - p.TT) * p.G : tk * p.G) + g;
     const long tok = cut.tok0 + tk;
     const int head = cut.hv * p.G + g;
-    join_row<DH, 4>(part_count(cut.parts), [&](int i) { return p.slot_ml + part_row(cut.parts, i, row) * 2; },
-                 [&](int i) { return p.slots + part_row(cut.parts, i, row) * DH; }, p.o + tok * p.ldo + (long)head * DH,
+    join_row<DH, 4>(part_count(cut.parts), [&](int i) { return p.slot_ml + part_row(cut.parts, i, row, blocks) * 2; },
+                 [&](int i) { return p.slots + part_row(cut.parts, i, row, blocks) * DH; }, p.o + tok * p.ldo + (long)head * DH,
                  p.lse != nullptr ? p.lse + tok * p.H + head : nullptr);
   }
 }
@@ -1060,25 +1064,26 @@ __global__ void __launch_bounds__(kJoinThreads, kCutBlocksPerSm) join_cut_tiles_
 // Every row of a batch that shares a prefix: its own parts and the prefix's. A whole tile's part lies
 // in the row buffers, a cut one's in the slots, at the row's place inside its tile.
 template <int DH>
-__global__ void __launch_bounds__(kJoinThreads) join_rows_kernel(PackedAttnParams p) {
+__global__ void __launch_bounds__(kJoinThreads) join_rows_kernel(PackedAttnParams p, int blocks) {
   wait_for_earlier_kernels();
   let_later_kernels_start();
   const long cls = (long)p.N * p.H, orow = (long)blockIdx.x * (kJoinThreads / 32) + (threadIdx.x >> 5);
   if (orow >= cls) return;
+  const bool failed = error_raised(p.err);
   const int own = p.row_parts[orow], pre = p.row_parts[cls + orow];
   const int tok = static_cast<int>(orow / p.H), head = static_cast<int>(orow - (long)tok * p.H);
-  if (tok < p.q_start[0] || tok >= p.q_start[p.B]) return;  // no request's row
+  if (failed || tok < p.q_start[0] || tok >= p.q_start[p.B]) return;  // no parts; no request's row
   auto whole = [](int parts) { return (parts & 0xffffff) == kWholeRow; };
   const int n_own = whole(own) ? 1 : part_count(own), n_pre = whole(pre) ? 1 : part_count(pre);
   const int own_row = static_cast<unsigned>(own) >> 24, pre_row = static_cast<unsigned>(pre) >> 24;
   join_row<DH, 8>(n_own + n_pre,
                [&](int i) -> const float* {
-                 if (i < n_own) return whole(own) ? p.row_ml + orow * 2 : p.slot_ml + part_row(own, i, own_row) * 2;
-                 return whole(pre) ? p.row_ml + (cls + orow) * 2 : p.slot_ml + part_row(pre, i - n_own, pre_row) * 2;
+                 if (i < n_own) return whole(own) ? p.row_ml + orow * 2 : p.slot_ml + part_row(own, i, own_row, blocks) * 2;
+                 return whole(pre) ? p.row_ml + (cls + orow) * 2 : p.slot_ml + part_row(pre, i - n_own, pre_row, blocks) * 2;
                },
                [&](int i) -> const float* {
-                 if (i < n_own) return whole(own) ? p.row_o + orow * DH : p.slots + part_row(own, i, own_row) * DH;
-                 return whole(pre) ? p.row_o + (cls + orow) * DH : p.slots + part_row(pre, i - n_own, pre_row) * DH;
+                 if (i < n_own) return whole(own) ? p.row_o + orow * DH : p.slots + part_row(own, i, own_row, blocks) * DH;
+                 return whole(pre) ? p.row_o + (cls + orow) * DH : p.slots + part_row(pre, i - n_own, pre_row, blocks) * DH;
                },
                p.o + (long)tok * p.ldo + (long)head * DH, p.lse != nullptr ? p.lse + orow : nullptr);
 }
@@ -1112,7 +1117,7 @@ void launch(const CUtensorMap& q, const CUtensorMap& q1, const CUtensorMap& k, c
   if (p.row_o != nullptr) {
     const long per = kJoinThreads / 32;
     cfg.gridDim = dim3(static_cast<unsigned>(((long)p.N * p.H + per - 1) / per));
-    cudaLaunchKernelEx(&cfg, join_rows_kernel<DH>, p);
+    cudaLaunchKernelEx(&cfg, join_rows_kernel<DH>, p, blocks);
   } else {
     cfg.gridDim = dim3(kCutBlocksPerSm * blocks);
     cudaLaunchKernelEx(&cfg, join_cut_tiles_kernel<DH>, p, blocks);

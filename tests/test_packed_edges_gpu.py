@@ -53,3 +53,25 @@ def test_slice_without_requests():
     b.at, b.own = b.at[:1], []
     run(b)
     assert bool((a.o == 7).all()) and bool((b.o == 7).all())
+
+
+# ------------------------------------------------------------------------------------ after an error
+@pytest.mark.parametrize("prefix", [0, 900])
+def test_no_rows_are_joined_after_an_error(prefix):
+    """An error that a kernel has recorded (its rows' parts may be missing): rows that would be joined stay
+    as they are, the host learns of it, and the next call is right."""
+    from appcorr_b200.ops.native import check_errors, err_word
+
+    c = Case([1], [6001], 28, 4, 128, prefix=prefix, seed=67)  # one tile a key head, cut over all SMs
+    err_word(torch.device(DEV)).fill_(2)
+    P, kw = _packed(), dict(q_start=_i(c.start), kv_len=_i(c.own), heads=28, kv_heads=4, head_dim=128, table=c.table, lse=c.lse)
+    if prefix:
+        P.shared_prefix_attention(c.q, c.k, c.v, c.o, prefix_table=c.prefix_table, prefix_len=prefix, **kw)
+    else:
+        P.packed_attention(c.q, c.k, c.v, c.o, **kw)
+    torch.cuda.synchronize()
+    assert bool((c.o == 7).all()) and bool((c.lse == 7).all())
+    with pytest.raises(RuntimeError, match="MMA wait timed out"):
+        check_errors(torch.device(DEV))
+    c.run()
+    c.check()
