@@ -77,7 +77,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch
     kv_len[b] packed rows of k / v from k_start[b]. Rows before q_start[0] or past q_start[B] are not
     touched (a call may take some of the batch's requests: slices of q_start, kv_len and table); a token
     that sees no key gets zeros (lse -inf). Cached rows past kv_len may hold anything. lse: fp32 [N, heads]
-    natural log-sum-exp of the scaled scores. scale: head_dim ** -0.5 by default."""
+    natural log-sum-exp of the scaled scores. scale: head_dim ** -0.5 by default; positive and finite."""
     _count(2)
     lib().packed_attention(q, k, v, o, q_start, kv_len, heads, kv_heads, head_dim,
                            head_dim ** -0.5 if scale is None else scale, table, k_start, None, 0, lse, _err(q))

@@ -3,6 +3,7 @@
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <cmath>
 #include <cudaTypedefs.h>
 
 #include "packed_attention.h"
@@ -55,6 +56,9 @@ void packed_attention_op(const at::Tensor& q, const at::Tensor& k, const at::Ten
                          c10::optional<at::Tensor> prefix_table, int64_t prefix_len, c10::optional<at::Tensor> lse, const at::Tensor& err) {
   APPCORR_CHECK(head_dim == 64 || head_dim == 128, "packed attention: head_dim must be 64 or 128, got ", head_dim);
   APPCORR_CHECK(heads > 0 && kv_heads > 0 && heads % kv_heads == 0, "packed attention: heads must be a multiple of kv_heads");
+  // the running maximum is that of the unscaled products, and what the mask hides is -inf before scaling
+  const float scale_log2 = static_cast<float>(scale * 1.4426950408889634);
+  APPCORR_CHECK(scale_log2 > 0.f && std::isfinite(scale_log2), "packed attention: scale must be positive and finite in fp32");
   pa_check_rows(q, "q", heads * head_dim);
   pa_check_rows(o, "o", heads * head_dim);
   pa_check_rows(k, "k", kv_heads * head_dim);
@@ -111,7 +115,7 @@ void packed_attention_op(const at::Tensor& q, const at::Tensor& k, const at::Ten
   p.kv_len = kv_len.data_ptr<int>();
   p.pages = static_cast<int>(k.size(0) / 128);
   p.key_rows = static_cast<int>(k.size(0));
-  p.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
+  p.scale_log2 = scale_log2;
   p.o = reinterpret_cast<__nv_bfloat16*>(o.data_ptr());
   p.ldo = o.size(0) > 1 ? o.stride(0) : heads * head_dim;
   p.err = err.data_ptr<int>();

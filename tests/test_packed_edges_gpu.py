@@ -75,3 +75,15 @@ def test_no_rows_are_joined_after_an_error(prefix):
         check_errors(torch.device(DEV))
     c.run()
     c.check()
+
+
+# ------------------------------------------------------------------------------------ arguments
+@pytest.mark.parametrize("prefix", [0, 200])
+def test_attention_refuses_scales_that_order_no_scores(prefix):
+    c = Case([2, 40], [2, 300], 4, 2, 64, prefix=prefix, seed=71)
+    for scale in (0.0, -0.125, 1e-60, 1e60, float("nan"), float("inf")):  # 1e-60 and 1e60 are 0 and infinite in fp32
+        with pytest.raises(RuntimeError, match="scale must be positive and finite"):
+            c.run(scale=scale)
+    assert bool((c.o == 7).all())
+    c.run(scale=1e-30)  # every visible key alike
+    c.check(scale=1e-30)
