@@ -77,16 +77,28 @@ class PackedAnswers:
         z = lambda n: torch.zeros(n, device=self.engine.device, dtype=torch.int32)  # noqa: E731
         self.held = z(self.max_requests)          # own tokens of each request so far
         self.free_at = z(2)                       # next free page, blocks that went without one
+        self.t["last"].zero_()                    # normalised last row of each request
 
     def step(self, ids: torch.Tensor, q_len: torch.Tensor) -> torch.Tensor:
-        """ids int32 [N]: the new tokens, request by request; q_len int32 [B] how many each brings (at
-        least one). -> fp32 logits [B, vocab] after each request's last token (valid until the next
-        step). Does not synchronise; `pages_missing` tells whether the pool was too small."""
+        """ids int32 [N]: the new tokens, request by request; q_len int32 [B] how many each brings.
+        -> fp32 logits [B, vocab] after each request's last token (valid until the next step). A request
+        that brings none (an answer that has ended) keeps those of its last step, zeros before its first.
+        Does not synchronise; `pages_missing` tells whether the pool was too small."""
         eng, c, t = self.engine, self.engine.cfg, self.t
         N, B = ids.numel(), q_len.numel()
         if N > self.max_step or B > self.max_requests:
             raise ValueError(f"{N} tokens of {B} requests: this batch holds {self.max_step} of {self.max_requests}")
-        dev = eng.device
+        if N:
+            self._layers(ids, q_len)
+        logits = t["logits"][:B]
+        if B:
+            K.gemm(t["last"][:B], eng.lm_head, logits, epi=K.EPI_F32)
+        return logits[:, :c.vocab]
+
+    def _layers(self, ids: torch.Tensor, q_len: torch.Tensor) -> None:
+        """The new tokens through every layer; `last` takes the last one of each request that brings any."""
+        eng, c, t = self.engine, self.engine.cfg, self.t
+        N, B = ids.numel(), q_len.numel()
         rows, req, pos, q_start = t["rows"][:N], t["req"][:N], t["pos"][:N], t["q_start"][:B + 1]
         kv_len, free_at = torch.empty_like(q_len), torch.empty_like(self.free_at)
         table = self.table[:B]
@@ -119,10 +131,9 @@ class PackedAnswers:
         self.held = torch.cat([kv_len, self.held[B:]])
         self.free_at = free_at
         last = t["last"][:B]
-        K.rmsnorm(x, eng.norm, c.rms_eps, last, rows=q_start[1:] - 1)
-        logits = t["logits"][:B]
-        K.gemm(last, eng.lm_head, logits, epi=K.EPI_F32)
-        return logits[:, :c.vocab]
+        ends = torch.empty_like(last)
+        K.rmsnorm(x, eng.norm, c.rms_eps, ends, rows=(q_start[1:] - 1).clamp(0, N - 1))
+        torch.where(q_len[:, None] > 0, ends, last, out=last)
 
     @property
     def pages_missing(self) -> int:

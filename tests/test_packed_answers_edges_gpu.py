@@ -1,0 +1,78 @@
+"""Packed answers (models/qwen_answers.py) at the edges of a step: requests that bring no token, lengths and
+ids that do not fit together, errors. The oracle and its tolerance are those of
+test_packed_answers_gpu.py."""
+import pytest
+import torch
+
+from test_packed_answers_gpu import DEV, _oracle, _rel, _setup
+
+pytestmark = pytest.mark.gpu
+
+
+def _ints(*values):
+    return torch.tensor(values, dtype=torch.int32, device=DEV)
+
+
+class Batch:
+    """Requests without an image, with their sequences beside them."""
+
+    def __init__(self, lengths, seed=5, **kw):
+        from appcorr_b200.models.qwen_answers import PackedAnswers
+
+        self.cfg, self.m, eng = _setup(seed=seed)
+        self.g = torch.Generator().manual_seed(seed + 4)
+        self.seqs = [torch.empty(0, dtype=torch.long, device=DEV) for _ in lengths]
+        self.pa = PackedAnswers(eng, **(dict(max_requests=len(lengths), max_own=200, max_step=256) | kw))
+        self.first = self.step(*lengths)
+
+    def step(self, *lengths):
+        new = [torch.randint(0, self.cfg.vocab, (n,), generator=self.g).to(DEV) for n in lengths]
+        out = self.pa.step(torch.cat(new).to(torch.int32), _ints(*lengths)).clone()
+        self.seqs = [torch.cat([s, x]) for s, x in zip(self.seqs, new)]
+        return out
+
+    def check(self, logits, b):
+        from appcorr_b200.ops.native import check_errors
+
+        torch.cuda.synchronize()
+        check_errors(torch.device(DEV))
+        s = self.seqs[b]
+        want = _oracle(self.m, self.m.embed_tokens(s), torch.arange(s.numel()).expand(3, -1))
+        assert _rel(logits[b], want) < 3e-2, b
+
+
+@pytest.mark.parametrize("idle", [(0,), (1,), (2,), (0, 1), (1, 2), (0, 2)])
+def test_requests_that_bring_no_token(idle):
+    """Their logits stay, the others go on, and they can go on later."""
+    t = Batch((40, 3, 150))
+    last = t.first
+    for n in (1, 2):
+        out = t.step(*(0 if b in idle else n for b in range(3)))
+        for b in range(3):
+            if b in idle:
+                assert torch.equal(out[b], last[b]), b
+            else:
+                t.check(out, b)
+    out = t.step(1, 1, 1)
+    for b in range(3):
+        t.check(out, b)
+
+
+def test_step_of_no_tokens_at_all():
+    t = Batch((40, 3, 150))
+    assert torch.equal(t.step(0, 0, 0), t.first)
+    out = t.step(2, 0, 1)
+    t.check(out, 0)
+    assert torch.equal(out[1], t.first[1])
+    assert t.pa.step(_ints(), _ints()).shape == (0, t.cfg.vocab)
+
+
+def test_request_that_has_not_begun():
+    """Zeros before its first token, also when the batch was used before."""
+    t = Batch((5, 0, 9))
+    assert bool((t.first[1] == 0).all())
+    t.check(t.first, 0)
+    t.check(t.first, 2)
+    t.step(1, 4, 0)
+    t.pa.reset()
+    assert bool((t.pa.step(_ints(3), _ints(1, 0, 0))[1:] == 0).all())
