@@ -78,18 +78,25 @@ class PackedAnswers:
         self.held = z(self.max_requests)          # own tokens of each request so far
         self.free_at = z(2)                       # next free page, blocks that went without one
         self.t["last"].zero_()                    # normalised last row of each request
+        self.short = torch.zeros((), device=self.engine.device, dtype=torch.int64)  # tokens that ids did not hold
 
     def step(self, ids: torch.Tensor, q_len: torch.Tensor) -> torch.Tensor:
         """ids int32 [N]: the new tokens, request by request; q_len int32 [B] how many each brings.
         -> fp32 logits [B, vocab] after each request's last token (valid until the next step). A request
         that brings none (an answer that has ended) keeps those of its last step, zeros before its first.
-        Does not synchronise; `pages_missing` tells whether the pool was too small."""
+        Tokens that q_len names and ids does not hold are not taken, ids past the sum of q_len are padding.
+        Does not synchronise; `tokens_missing` tells whether ids were too few, `pages_missing` whether the
+        pool was too small."""
         eng, c, t = self.engine, self.engine.cfg, self.t
         N, B = ids.numel(), q_len.numel()
         if N > self.max_step or B > self.max_requests:
             raise ValueError(f"{N} tokens of {B} requests: this batch holds {self.max_step} of {self.max_requests}")
+        ends = q_len.clamp(min=0).cumsum(0)
+        held = torch.nn.functional.pad(ends.clamp(max=N), (1, 0))  # of each request, the tokens that are there
+        if B:
+            self.short += ends[-1] - held[-1]
         if N:
-            self._layers(ids, q_len)
+            self._layers(ids, held.diff().to(torch.int32))
         logits = t["logits"][:B]
         if B:
             K.gemm(t["last"][:B], eng.lm_head, logits, epi=K.EPI_F32)
@@ -139,6 +146,11 @@ class PackedAnswers:
     def pages_missing(self) -> int:
         """Blocks that went without a page so far (synchronises); above zero the answers are not valid."""
         return int(self.free_at[1])
+
+    @property
+    def tokens_missing(self) -> int:
+        """Tokens named by q_len that ids did not hold so far (synchronises)."""
+        return int(self.short)
 
     def generate(self, questions: List[torch.Tensor], n: int) -> torch.Tensor:
         """Greedy answers of n tokens to the questions (int32 token ids each) -> int32 [B, n]."""

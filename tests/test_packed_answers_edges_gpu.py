@@ -76,3 +76,22 @@ def test_request_that_has_not_begun():
     t.step(1, 4, 0)
     t.pa.reset()
     assert bool((t.pa.step(_ints(3), _ints(1, 0, 0))[1:] == 0).all())
+
+
+def test_lengths_and_ids_that_do_not_fit():
+    """Tokens that ids does not hold are not taken, and counted; ids past the lengths are padding."""
+    t = Batch((40, 3, 150))
+    ids = torch.randint(0, t.cfg.vocab, (7,), generator=t.g).to(device=DEV, dtype=torch.int32)
+    for lengths, taken in (((2, 9, 4), (2, 5, 0)), ((7, 1, 1), (7, 0, 0)), ((1 << 30, 1 << 30, 1 << 30), (7, 0, 0)), ((1, 2, 1), (1, 2, 1)),
+                           ((-3, 2, 5), (0, 2, 5))):
+        missing = t.pa.tokens_missing
+        out = t.pa.step(ids, _ints(*lengths)).clone()
+        at = 0
+        for b, n in enumerate(taken):
+            t.seqs[b] = torch.cat([t.seqs[b], ids[at:at + n].long()])
+            at += n
+            t.check(out, b)
+        assert t.pa.tokens_missing - missing == max(sum(max(n, 0) for n in lengths) - 7, 0)
+        assert t.pa.held.tolist() == [s.numel() for s in t.seqs]
+    assert t.pa.pages_missing == 0
+    assert t.pa.step(_ints(), _ints(0, 2, 0)).shape[0] == 3 and t.pa.held.tolist() == [s.numel() for s in t.seqs]
