@@ -81,13 +81,17 @@ class PackedAnswers:
         self.short = torch.zeros((), device=self.engine.device, dtype=torch.int64)  # tokens that ids did not hold
 
     def step(self, ids: torch.Tensor, q_len: torch.Tensor) -> torch.Tensor:
-        """ids int32 [N]: the new tokens, request by request; q_len int32 [B] how many each brings.
+        """ids int32 (N values): the new tokens, request by request; q_len int32 [B] how many each brings.
+        Both lie on the engine's device; ids are rows of the embedding and not checked against it here.
         -> fp32 logits [B, vocab] after each request's last token (valid until the next step). A request
         that brings none (an answer that has ended) keeps those of its last step, zeros before its first.
         Tokens that q_len names and ids does not hold are not taken, ids past the sum of q_len are padding.
         Does not synchronise; `tokens_missing` tells whether ids were too few, `pages_missing` whether the
         pool was too small."""
         eng, c, t = self.engine, self.engine.cfg, self.t
+        for name, x, fits in (("ids", ids, ids.is_contiguous()), ("q_len", q_len, q_len.dim() == 1)):
+            if x.dtype != torch.int32 or x.device != t["x"].device or not fits:
+                raise ValueError(f"{name} must be int32 on {t['x'].device}, ids contiguous, q_len of one dimension")
         N, B = ids.numel(), q_len.numel()
         if N > self.max_step or B > self.max_requests:
             raise ValueError(f"{N} tokens of {B} requests: this batch holds {self.max_step} of {self.max_requests}")
@@ -157,8 +161,12 @@ class PackedAnswers:
         dev = self.engine.device
         if not questions or any(q.numel() == 0 for q in questions):
             raise ValueError("every request needs at least one token")
+        ids = torch.cat([q.to(device=dev, dtype=torch.int64).reshape(-1) for q in questions])
+        lo, hi = (int(v) for v in torch.stack(ids.aminmax()))
+        if lo < 0 or hi >= self.engine.cfg.vocab:
+            raise ValueError(f"token ids from {lo} to {hi}: the vocabulary has {self.engine.cfg.vocab}")
+        ids = ids.to(torch.int32)
         self.reset()
-        ids = torch.cat([q.to(device=dev, dtype=torch.int32).reshape(-1) for q in questions])
         q_len = torch.tensor([q.numel() for q in questions], dtype=torch.int32, device=dev)
         one = torch.ones_like(q_len)
         out = []

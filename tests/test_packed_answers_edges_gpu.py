@@ -95,3 +95,20 @@ def test_lengths_and_ids_that_do_not_fit():
         assert t.pa.held.tolist() == [s.numel() for s in t.seqs]
     assert t.pa.pages_missing == 0
     assert t.pa.step(_ints(), _ints(0, 2, 0)).shape[0] == 3 and t.pa.held.tolist() == [s.numel() for s in t.seqs]
+
+
+def test_ids_that_are_no_rows_of_the_embedding_are_refused():
+    """On the host, of another type or stride, outside the vocabulary: nothing runs, nothing is forgotten."""
+    t = Batch((40, 3, 150))
+    one, vocab = _ints(1, 1, 1), t.cfg.vocab
+    for ids, q_len in ((_ints(1, 2, 3).cpu(), one), (_ints(1, 2, 3).long(), one), (_ints(1, 9, 2, 9, 3, 9)[::2], one),
+                       (_ints(1, 2, 3), one.cpu()), (_ints(1, 2, 3), one.long()), (_ints(1, 2, 3), one[None])):
+        with pytest.raises(ValueError, match="must be int32"):
+            t.pa.step(ids, q_len)
+    for ids in (_ints(1, vocab), _ints(-1, 1), torch.tensor([vocab]), torch.tensor([(1 << 32) + 5])):
+        with pytest.raises(ValueError, match="vocabulary"):
+            t.pa.generate([_ints(1), ids], 2)
+    assert t.pa.held.tolist() == [40, 3, 150]
+    out = t.pa.step(_ints(1, 2, 3)[None], _ints(1, 9, 1, 9, 1, 9)[::2])  # shapes that make no difference
+    t.seqs[1] = torch.cat([t.seqs[1], _ints(2).long()])
+    t.check(out, 1)
