@@ -23,6 +23,7 @@ import torch
 
 from ..ops import kernels as K
 from ..ops import packed as P
+from ..ops.native import check_errors
 from .qwen_engine import BF16, QwenSession, QwenVLEngine, _pad_to
 
 
@@ -157,7 +158,8 @@ class PackedAnswers:
         return int(self.short)
 
     def generate(self, questions: List[torch.Tensor], n: int) -> torch.Tensor:
-        """Greedy answers of n tokens to the questions (int32 token ids each) -> int32 [B, n]."""
+        """Greedy answers of n tokens to the questions (int32 token ids each) -> int32 [B, n]. Raises where
+        a kernel has recorded an error or the pages did not do (synchronises)."""
         dev = self.engine.device
         if not questions or any(q.numel() == 0 for q in questions):
             raise ValueError("every request needs at least one token")
@@ -174,6 +176,7 @@ class PackedAnswers:
             ids = self.step(ids, q_len).argmax(1).to(torch.int32)
             out.append(ids)
             q_len = one
+        check_errors(dev)
         if self.pages_missing:
             raise RuntimeError("PackedAnswers: the requests outgrew the page pool (max_own)")
         return torch.stack(out, 1)

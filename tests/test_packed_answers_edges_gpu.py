@@ -112,3 +112,24 @@ def test_ids_that_are_no_rows_of_the_embedding_are_refused():
     out = t.pa.step(_ints(1, 2, 3)[None], _ints(1, 9, 1, 9, 1, 9)[::2])  # shapes that make no difference
     t.seqs[1] = torch.cat([t.seqs[1], _ints(2).long()])
     t.check(out, 1)
+
+
+def test_generate_raises_recorded_errors():
+    from appcorr_b200.ops.native import err_word
+
+    t = Batch((4, 3))
+    questions = [_ints(1, 2), _ints(3)]
+    want, step, calls = t.pa.generate(questions, 3), t.pa.step, []
+
+    def last_step_fails(ids, q_len):
+        out = step(ids, q_len)
+        calls.append(1)
+        if len(calls) == 3:
+            err_word(torch.device(DEV)).fill_(3)
+        return out
+
+    t.pa.step = last_step_fails
+    with pytest.raises(RuntimeError, match="epilogue wait timed out"):
+        t.pa.generate(questions, 3)
+    t.pa.step = step
+    assert torch.equal(t.pa.generate(questions, 3), want)
