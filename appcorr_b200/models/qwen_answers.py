@@ -163,6 +163,8 @@ class PackedAnswers:
         dev = self.engine.device
         if not questions or any(q.numel() == 0 for q in questions):
             raise ValueError("every request needs at least one token")
+        if n < 0:
+            raise ValueError(f"answers of {n} tokens")
         ids = torch.cat([q.to(device=dev, dtype=torch.int64).reshape(-1) for q in questions])
         lo, hi = (int(v) for v in torch.stack(ids.aminmax()))
         if lo < 0 or hi >= self.engine.cfg.vocab:
@@ -179,4 +181,4 @@ class PackedAnswers:
         check_errors(dev)
         if self.pages_missing:
             raise RuntimeError("PackedAnswers: the requests outgrew the page pool (max_own)")
-        return torch.stack(out, 1)
+        return torch.stack(out, 1) if out else ids.new_empty(len(questions), 0)

@@ -133,3 +133,11 @@ def test_generate_raises_recorded_errors():
         t.pa.generate(questions, 3)
     t.pa.step = step
     assert torch.equal(t.pa.generate(questions, 3), want)
+
+
+def test_generate_no_tokens():
+    t = Batch((4, 3))
+    out = t.pa.generate([_ints(1, 2), _ints(3)], 0)
+    assert out.shape == (2, 0) and out.dtype == torch.int32 and out.device == t.pa.held.device
+    with pytest.raises(ValueError, match="-1 tokens"):
+        t.pa.generate([_ints(1)], -1)
