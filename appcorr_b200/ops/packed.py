@@ -44,8 +44,8 @@ def packed_layout(q_len: torch.Tensor, past: torch.Tensor, table: torch.Tensor, 
     rows / req / pos [N]: cache row, request and position of every token; N may exceed the sum of
     q_len (a fixed-size batch), the tokens past it get -1. free_next [2]: the index of the first page
     still free, and how many blocks went without a page (free list or table too short): their
-    table entries and their tokens' rows are -1. free_next may not be free_start itself; give a step
-    the last one's free_next[:1] to carry on."""
+    table entries and their tokens' rows are -1; give a step the last one's free_next[:1] to carry on.
+    No output may lie in the place of an input or of another output."""
     _count()
     lib().packed_layout(q_len, past, table, free_pages, free_start, q_start, kv_len, rows, req, pos, free_next)
 

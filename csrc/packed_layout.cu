@@ -169,10 +169,34 @@ void packed_layout_op(const at::Tensor& q_len, const at::Tensor& past, at::Tenso
                               (const at::Tensor*)&kv_len, (const at::Tensor*)&rows, (const at::Tensor*)&req,
                               (const at::Tensor*)&pos, (const at::Tensor*)&free_next})
     APPCORR_CHECK(t->device() == q_len.device(), "packed_layout: tensors on different devices");
-  APPCORR_CHECK(free_next.data_ptr() != free_start.data_ptr(),
-              "packed_layout: free_next must not be free_start (every block reads it)");
-  APPCORR_CHECK(B == 0 || (kv_len.data_ptr() != past.data_ptr() && kv_len.data_ptr() != q_len.data_ptr()),
-                "packed_layout: kv_len must not be past or q_len (every block reads them)");
+  // every block reads the inputs while others write the outputs: no output in the place of an input or
+  // of another output, as far as they are read and written
+  const int64_t W = table.size(1), ld = B > 1 ? table.stride(0) : W;
+  APPCORR_CHECK(ld >= W, "packed_layout: the rows of table overlap");
+  struct Part {
+    const char* name;
+    const int *from, *to;
+  };
+  auto part = [](const char* name, const at::Tensor& t, int64_t n) { return Part{name, t.data_ptr<int>(), t.data_ptr<int>() + n}; };
+  const Part in[] = {part("q_len", q_len, B), part("past", past, B), part("free_pages", free_pages, free_pages.numel()),
+                     part("free_start", free_start, 1)};
+  const Part out[] = {part("q_start", q_start, B + 1), part("kv_len", kv_len, B), part("rows", rows, N),
+                      part("req", req, N),             part("pos", pos, N),       part("free_next", free_next, 2)};
+  auto meet = [](const Part& a, const Part& b) { return a.from < b.to && b.from < a.to && a.from < a.to && b.from < b.to; };
+  auto meets_table = [&](const Part& a) {
+    if (a.from == a.to || B == 0 || W == 0) return false;
+    const int64_t lo = a.from - table.data_ptr<int>(), hi = lo + (a.to - a.from);
+    const int64_t r = lo < W ? 0 : (lo - W) / ld + 1;  // the first row that ends after lo
+    return r < B && r * ld < hi;
+  };
+  for (const Part& a : out) {
+    for (const Part& b : in)
+      APPCORR_CHECK(!meet(a, b), "packed_layout: ", a.name, " must not lie in the place of ", b.name);
+    for (const Part& b : out)
+      APPCORR_CHECK(&a == &b || !meet(a, b), "packed_layout: ", a.name, " must not lie in the place of ", b.name);
+    APPCORR_CHECK(!meets_table(a), "packed_layout: ", a.name, " must not lie in the place of table");
+  }
+  for (const Part& b : in) APPCORR_CHECK(!meets_table(b), "packed_layout: table must not lie in the place of ", b.name);
   c10::cuda::CUDAGuard guard(q_len.device());
   LayoutParams p{q_len.data_ptr<int>(), past.data_ptr<int>(), table.data_ptr<int>(), table.stride(0),
                  free_pages.data_ptr<int>(), free_start.data_ptr<int>(), q_start.data_ptr<int>(), kv_len.data_ptr<int>(),

@@ -87,3 +87,52 @@ def test_attention_refuses_scales_that_order_no_scores(prefix):
     assert bool((c.o == 7).all())
     c.run(scale=1e-30)  # every visible key alike
     c.check(scale=1e-30)
+
+
+def _layout_args(B=3, N=5, W=4):
+    e = lambda *n: torch.zeros(*n, dtype=torch.int32, device=DEV)  # noqa: E731
+    return dict(q_len=e(B), past=e(B), table=e(B, W), free_pages=e(9), free_start=e(1), q_start=e(B + 1), kv_len=e(B), rows=e(N), req=e(N),
+                pos=e(N), free_next=e(2))
+
+
+LAYOUT_IN, LAYOUT_OUT = ("q_len", "past", "free_pages", "free_start", "table"), ("q_start", "kv_len", "rows", "req", "pos", "free_next")
+
+
+def _layout_call(a):
+    _packed().packed_layout(*(a[k] for k in ("q_len", "past", "table", "free_pages", "free_start")), **{k: a[k] for k in LAYOUT_OUT})
+
+
+def _in_one_buffer(a, first, second, gap):
+    """The two arguments as views of one buffer, the second `gap` values after the first one's begin."""
+    n, m = a[first].numel(), a[second].numel()
+    buf = torch.zeros(n + m + gap + 8, dtype=torch.int32, device=DEV)
+    return {**a, first: buf[:n].view(a[first].shape), second: buf[gap:gap + m].view(a[second].shape)}
+
+
+@pytest.mark.parametrize("out", LAYOUT_OUT)
+def test_layout_refuses_outputs_in_place_of_other_arguments(out):
+    for other in LAYOUT_IN + LAYOUT_OUT:
+        if other == out:
+            continue
+        a = _layout_args()
+        for first, second in ((out, other), (other, out)):
+            for gap in (0, a[first].numel() - 1):  # the same place; one value in common
+                with pytest.raises(RuntimeError, match="must not lie in the place of"):
+                    _layout_call(_in_one_buffer(a, first, second, gap))
+            _layout_call(_in_one_buffer(a, first, second, a[first].numel()))  # side by side
+    _done()
+
+
+def test_layout_overlaps_of_the_table():
+    """What lies between the table's rows or behind those that are used is no part of it."""
+    buf = torch.zeros(6, 9, dtype=torch.int32, device=DEV)
+    a = _layout_args() | dict(table=buf[:, :4])
+    _layout_call(a | dict(kv_len=buf[1, 4:7], q_start=buf[2, 5:9], free_next=buf[3, :2], q_len=buf[4, :3], past=buf[0, 6:9]))
+    for kw in (dict(kv_len=buf[1, 3:6]), dict(q_start=buf[1, 6:10].new_zeros(0).set_(buf.untyped_storage(), 15, (4,))), dict(past=buf[2, :3]),
+               dict(free_pages=buf.view(-1)[40 - 22:40 - 22 + 9]), dict(free_next=buf[0, 3:5]),
+               dict(table=torch.zeros(4, dtype=torch.int32, device=DEV).expand(3, 4))):
+        with pytest.raises(RuntimeError, match="must not lie in the place of|overlap"):
+            _layout_call(a | kw)
+    one = _layout_args(B=1) | dict(table=buf[:1, :9])
+    _layout_call(one | dict(kv_len=buf[1, :1]))
+    _done()
