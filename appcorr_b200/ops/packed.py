@@ -41,8 +41,8 @@ def packed_layout(q_len: torch.Tensor, past: torch.Tensor, table: torch.Tensor, 
     q_start [B + 1]: first packed row of each request. kv_len [B] = past + q_len. table [>= B, W]:
     each request's pages; the entries of blocks that `past` filled are read, those of the blocks this
     step adds are written with free_pages[free_start[0]], the next one, ..., in request order.
-    rows / req / pos [N]: cache row, request and position of every token; N may exceed the sum of
-    q_len (a fixed-size batch), the tokens past it get -1. free_next [2]: the index of the first page
+    rows / req / pos [N]: cache row, request and position of every token (row -1 where its page is below
+    zero or 2^24 and more); N may exceed the sum of q_len (a fixed-size batch), the tokens past it get -1. free_next [2]: the index of the first page
     still free, and how many blocks went without a page (free list or table too short): their
     table entries and their tokens' rows are -1; give a step the last one's free_next[:1] to carry on.
     No output may lie in the place of an input or of another output."""

@@ -26,6 +26,7 @@ namespace appcorr {
 
 constexpr int kPlRows = 128;      // rows per cache page
 constexpr int kPlThreads = 1024;  // requests scanned at a time
+constexpr unsigned kPlPages = (1u << 31) / kPlRows;  // pages whose rows have 32-bit numbers
 
 struct LayoutParams {
   const int* q_len;
@@ -124,7 +125,7 @@ __global__ void __launch_bounds__(kPlThreads) packed_layout_kernel(LayoutParams 
           if (src < p.F) page = p.free_pages[src];
         }
       }
-      p.rows[n] = page >= 0 ? page * kPlRows + at % kPlRows : -1;
+      p.rows[n] = static_cast<unsigned>(page) < kPlPages ? page * kPlRows + at % kPlRows : -1;
       p.req[n] = b0 + lo;
       p.pos[n] = at;
     }

@@ -4,7 +4,7 @@ test_packed_gpu.py, whose cases and 64-bit statements are used here."""
 import pytest
 import torch
 
-from test_packed_gpu import DEV, Case, _done, _i, _packed
+from test_packed_gpu import DEV, Case, _done, _i, _layout_plain, _layout_run, _packed
 
 pytestmark = pytest.mark.gpu
 
@@ -136,3 +136,16 @@ def test_layout_overlaps_of_the_table():
     one = _layout_args(B=1) | dict(table=buf[:1, :9])
     _layout_call(one | dict(kv_len=buf[1, :1]))
     _done()
+
+
+# ------------------------------------------------------------------------------------ values on the device
+def test_layout_pages_without_rows():
+    """A page number whose rows pass 32 bits is no page: its tokens get row -1, not some other page's row."""
+    q, past = [4, 2, 1, 260, 3], [127, 200, 0, 0, 253]
+    table = [[1 << 24, 5, 5], [3, 1 << 25, 5], [5, 5, 5], [5, 5, 5], [5, (1 << 24) - 1, 5]]
+    free = [(1 << 30) + 1, 1 << 24, 7, -9]
+    got = _layout_run(q, past, table, free, 0)
+    want = _layout_plain(q, past, table, free, 0)
+    want["rows"] = [r if r < 1 << 31 else -1 for r in want["rows"]]
+    assert want["rows"].count(-1) == 4 + 2 + 1 + 132 and want["rows"][-1] == (1 << 31) - 1
+    assert got == want
