@@ -38,7 +38,8 @@ def packed_layout(q_len: torch.Tensor, past: torch.Tensor, table: torch.Tensor, 
                   req: torch.Tensor, pos: torch.Tensor, free_next: torch.Tensor) -> None:
     """Layout of one step (int32 throughout): q_len [B] new tokens after past [B] cached ones.
 
-    q_start [B + 1]: first packed row of each request. kv_len [B] = past + q_len. table [>= B, W]:
+    q_start [B + 1]: first packed row of each request (the sum of q_len stays below 2^31; a length below
+    zero counts as zero). kv_len [B] = past + q_len, at most 2^31 - 1, like pos. table [>= B, W]:
     each request's pages; the entries of blocks that `past` filled are read, those of the blocks this
     step adds are written with free_pages[free_start[0]], the next one, ..., in request order.
     rows / req / pos [N]: cache row, request and position of every token (row -1 where its page is below

@@ -44,6 +44,10 @@ struct LayoutParams {
   int B, W, F, N;
 };
 
+// past + q_len passes 31 bits where a length is near 2^31, and is kept in unsigned 32 bits
+__device__ __forceinline__ int blocks_of(unsigned rows) { return static_cast<int>(rows / kPlRows + (rows % kPlRows != 0)); }
+__device__ __forceinline__ int capped(unsigned n) { return static_cast<int>(min(n, 0x7fffffffu)); }
+
 __global__ void __launch_bounds__(kPlThreads) packed_layout_kernel(LayoutParams p) {
   __shared__ int s_start[kPlThreads + 1], s_past[kPlThreads], s_first[kPlThreads];
   __shared__ int s_warp[3][32];
@@ -55,7 +59,7 @@ __global__ void __launch_bounds__(kPlThreads) packed_layout_kernel(LayoutParams 
   for (int b0 = 0; b0 < p.B; b0 += kPlThreads) {
     const int b = b0 + tid, nb = min(kPlThreads, p.B - b0);
     const int q = b < p.B ? max(p.q_len[b], 0) : 0, past = b < p.B ? max(p.past[b], 0) : 0;
-    const int have = (past + kPlRows - 1) / kPlRows, total = (past + q + kPlRows - 1) / kPlRows;
+    const int have = blocks_of(past), total = blocks_of((unsigned)past + q);
     const int need = max(min(total, p.W) - have, 0), over = max(total - max(p.W, have), 0);
     // three inclusive scans at once: tokens, new pages, blocks past the table's width
     int v[3] = {q, need, over};
@@ -93,48 +97,48 @@ __global__ void __launch_bounds__(kPlThreads) packed_layout_kernel(LayoutParams 
     if (tid == 0) s_start[nb] = tok_end;
     if (blockIdx.x == 0 && b < p.B) {
       p.q_start[b] = tok;
-      p.kv_len[b] = past + q;
+      p.kv_len[b] = capped((unsigned)past + q);
     }
     __syncthreads();
     // new pages of this block's requests: one warp each
     for (int r = blockIdx.x + gridDim.x * warp; r < nb; r += gridDim.x * (kPlThreads / 32)) {
-      const int pst = s_past[r], ql = s_start[r + 1] - s_start[r];
-      const int hv = (pst + kPlRows - 1) / kPlRows;
-      const int nd = min((pst + ql + kPlRows - 1) / kPlRows, p.W) - hv;
+      const unsigned pst = s_past[r], ql = (unsigned)s_start[r + 1] - s_start[r];
+      const int hv = blocks_of(pst);
+      const int nd = min(blocks_of(pst + ql), p.W) - hv;
       for (int i = lane; i < nd; i += 32) {
-        const long src = (long)begin + s_first[r] + i;
+        const unsigned long src = (long)begin + s_first[r] + i;
         p.table[(b0 + r) * p.ld_table + hv + i] = src < p.F ? p.free_pages[src] : -1;
       }
     }
     // this block's tokens inside the chunk
-    for (int n = max(n0, tok_base) + tid; n < min(n1, tok_end); n += kPlThreads) {
+    for (int n = max(n0, min(tok_base, n1)) + tid; n < min(n1, tok_end); n += kPlThreads) {
       int lo = 0, hi = nb;  // the last request that starts at or before n (empty ones lie before it)
       while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
         if (s_start[mid] <= n) lo = mid;
         else hi = mid;
       }
-      const int pst = s_past[lo], at = pst + n - s_start[lo], blk = at / kPlRows;
-      const int hv = (pst + kPlRows - 1) / kPlRows;
+      const unsigned pst = s_past[lo], at = pst + n - s_start[lo];
+      const int blk = at / kPlRows, hv = blocks_of(pst);
       int page = -1;
       if (blk < p.W) {
         if (blk < hv) {
           page = p.table[(b0 + lo) * p.ld_table + blk];
         } else {
-          const long src = (long)begin + s_first[lo] + blk - hv;
+          const unsigned long src = (long)begin + s_first[lo] + blk - hv;
           if (src < p.F) page = p.free_pages[src];
         }
       }
       p.rows[n] = static_cast<unsigned>(page) < kPlPages ? page * kPlRows + at % kPlRows : -1;
       p.req[n] = b0 + lo;
-      p.pos[n] = at;
+      p.pos[n] = capped(at);
     }
     tok_base = tok_end;
     page_base = page_end;
     over_base = over_end;
     __syncthreads();
   }
-  for (int n = max(n0, tok_base) + tid; n < n1; n += kPlThreads) p.rows[n] = p.req[n] = p.pos[n] = -1;  // padding
+  for (int n = max(n0, min(tok_base, n1)) + tid; n < n1; n += kPlThreads) p.rows[n] = p.req[n] = p.pos[n] = -1;  // padding
   if (blockIdx.x == 0 && tid == 0) {
     p.q_start[p.B] = tok_base;
     const long end = (long)begin + page_base, given = min(end, (long)max(p.F, begin));
@@ -165,7 +169,8 @@ void packed_layout_op(const at::Tensor& q_len, const at::Tensor& past, at::Tenso
   check_i32(pos, "pos", 1, N);
   check_i32(free_next, "free_next", 1, 2);
   APPCORR_CHECK(table.size(0) >= B, "packed_layout: table has ", table.size(0), " rows for ", B, " requests");
-  APPCORR_CHECK(N < (int64_t(1) << 31) && B < (int64_t(1) << 31) - kPlThreads, "packed_layout: too many tokens or requests");
+  constexpr int64_t kMost = (int64_t(1) << 31) - 2 * kPlThreads;  // a block's next token or request still has a 32-bit number
+  APPCORR_CHECK(N < kMost && B < kMost, "packed_layout: too many tokens or requests");
   for (const at::Tensor* t : {&past, (const at::Tensor*)&table, &free_pages, &free_start, (const at::Tensor*)&q_start,
                               (const at::Tensor*)&kv_len, (const at::Tensor*)&rows, (const at::Tensor*)&req,
                               (const at::Tensor*)&pos, (const at::Tensor*)&free_next})

@@ -149,3 +149,37 @@ def test_layout_pages_without_rows():
     want["rows"] = [r if r < 1 << 31 else -1 for r in want["rows"]]
     assert want["rows"].count(-1) == 4 + 2 + 1 + 132 and want["rows"][-1] == (1 << 31) - 1
     assert got == want
+
+
+TOP = (1 << 31) - 1
+
+
+@pytest.mark.parametrize("past", [TOP, TOP - 1, TOP - 126, TOP - 127, TOP - 128, TOP - 199, TOP - 200, TOP - 201, 1 << 30])
+def test_layout_lengths_whose_sum_passes_32_bits(past):
+    """Such requests get neither pages nor rows; those beside them are laid out, and nothing else is written."""
+    q, pasts = [3, 200, 130], [126, past, 5]
+    buf = torch.full((3, 3, 4), -7, dtype=torch.int32, device=DEV)
+    buf[1, :, 0] = _i([20, 21, 22])
+    out = {k: torch.full((n,), 77, dtype=torch.int32, device=DEV) for k, n in (("q_start", 4), ("kv_len", 3), ("rows", 333), ("req", 333), ("pos", 333), ("free_next", 2))}
+    _packed().packed_layout(_i(q), _i(pasts), buf[1], _i([5, 6, 7]), _i([0]), **out)
+    _done()
+    want_kv = [129, min(past + 200, TOP), 135]
+    blocks = -(-(past + 200) // 128) - -(-past // 128)
+    assert out["q_start"].tolist() == [0, 3, 203, 333] and out["kv_len"].tolist() == want_kv
+    assert buf[1].tolist() == [[20, 5, -7, -7], [21, -7, -7, -7], [22, 6, -7, -7]] and bool((buf[::2] == -7).all())
+    assert out["rows"].tolist() == [20 * 128 + 126, 20 * 128 + 127, 5 * 128] + [-1] * 200 + list(range(22 * 128 + 5, 23 * 128)) + list(range(6 * 128, 6 * 128 + 7))
+    assert out["req"].tolist() == [0] * 3 + [1] * 200 + [2] * 130
+    assert out["pos"].tolist() == [126, 127, 128] + [min(past + i, TOP) for i in range(200)] + list(range(5, 135))
+    assert out["free_next"].tolist() == [2, blocks]
+
+
+def test_layout_lengths_of_the_largest_kind():
+    """Lengths of 2^31 - 1 beside short ones, negative lengths: what fits the table and the batch is right."""
+    out = {k: torch.full((n,), 77, dtype=torch.int32, device=DEV) for k, n in (("q_start", 4), ("kv_len", 3), ("rows", 40), ("req", 40), ("pos", 40), ("free_next", 2))}
+    table = torch.full((3, 2), -7, dtype=torch.int32, device=DEV)
+    _packed().packed_layout(_i([30, -5, TOP - 30]), _i([-1, 200, TOP]), table, _i([4, 5, 6]), _i([0]), **out)
+    _done()
+    assert out["q_start"].tolist() == [0, 30, 30, TOP] and out["kv_len"].tolist() == [30, 200, TOP]
+    assert table.tolist() == [[4, -7], [-7, -7], [-7, -7]]
+    assert out["rows"].tolist() == list(range(4 * 128, 4 * 128 + 30)) + [-1] * 10 and out["pos"][30:].tolist() == [TOP] * 10
+    assert out["req"].tolist() == [0] * 30 + [2] * 10
