@@ -45,7 +45,7 @@ static void pa_check_rows(const at::Tensor& t, const char* name, int64_t width) 
               "packed attention: ", name, " rows must be 16-byte aligned and must not overlap");
 }
 static void pa_check_i32(const at::Tensor& t, const char* name, int64_t dim, int64_t least) {
-  APPCORR_CHECK(t.is_cuda() && t.scalar_type() == at::kInt && t.dim() == dim && t.stride(-1) == 1 && t.numel() >= least,
+  APPCORR_CHECK(t.is_cuda() && t.scalar_type() == at::kInt && t.dim() == dim && (t.size(-1) <= 1 || t.stride(-1) == 1) && t.numel() >= least,
               "packed attention: ", name, " must be a CUDA int32 tensor of ", dim, " dimension(s), unit inner stride and at least ",
               least, " values");
 }

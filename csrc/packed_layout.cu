@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(kPlThreads) packed_layout_kernel(LayoutParams 
 }
 
 static void check_i32(const at::Tensor& t, const char* name, int64_t dim, int64_t least) {
-  APPCORR_CHECK(t.is_cuda() && t.scalar_type() == at::kInt && t.dim() == dim && t.stride(-1) == 1, "packed_layout: ", name,
+  APPCORR_CHECK(t.is_cuda() && t.scalar_type() == at::kInt && t.dim() == dim && (t.size(-1) <= 1 || t.stride(-1) == 1), "packed_layout: ", name,
               " must be a CUDA int32 tensor of ", dim, " dimension(s) with unit inner stride");
   APPCORR_CHECK(t.numel() >= least, "packed_layout: ", name, " holds ", t.numel(), " values, ", least, " are needed");
 }

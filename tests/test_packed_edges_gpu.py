@@ -183,3 +183,21 @@ def test_layout_lengths_of_the_largest_kind():
     assert table.tolist() == [[4, -7], [-7, -7], [-7, -7]]
     assert out["rows"].tolist() == list(range(4 * 128, 4 * 128 + 30)) + [-1] * 10 and out["pos"][30:].tolist() == [TOP] * 10
     assert out["req"].tolist() == [0] * 30 + [2] * 10
+
+
+# ------------------------------------------------------------------------------------ strides
+def test_single_values_of_any_stride():
+    """One value, or one column, has no inner stride (torch calls it contiguous whatever it is)."""
+    one = lambda v: torch.full((1, 3), v, dtype=torch.int32, device=DEV)[:, 0]  # noqa: E731
+    assert one(1).stride() == (3,) and one(1).is_contiguous() and _i([[1, 2]]).T[:1].stride(1) == 2
+    a = _layout_args(B=1, N=2, W=1) | dict(q_len=one(2), past=one(3), kv_len=one(0), free_start=one(0), free_pages=one(9), table=_i([[4, 2]]).T[:1])
+    _layout_call(a)
+    _done()
+    assert a["kv_len"].tolist() == [5] and a["rows"].tolist() == [4 * 128 + 3, 4 * 128 + 4] and a["pos"].tolist() == [3, 4]
+    c = Case([2], [100], 4, 2, 64, seed=73)
+    c.run(kv_len=one(100), table=torch.cat([c.table[:, :1]] * 2, 1).T[:1])
+    c.check()
+    c = Case([2], [100], 4, 2, 64, seed=73, prefix=5)
+    c.prefix_table = torch.stack([c.prefix_table] * 2, 1)[:, 0]
+    c.run(kv_len=one(100))
+    c.check()
