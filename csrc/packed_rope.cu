@@ -163,6 +163,10 @@ static void check_rows_bf16(const at::Tensor& t, const char* name, int64_t width
   APPCORR_CHECK((t.size(0) <= 1 || t.stride(0) % 8 == 0) && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0,
               "qk_norm_rope: ", name, " rows must be 16-byte aligned");
 }
+static void check_written_rows(const at::Tensor& t, const char* name, int64_t width) {
+  check_rows_bf16(t, name, width);
+  APPCORR_CHECK(t.size(0) <= 1 || t.stride(0) >= width, "qk_norm_rope: ", name, " rows must not overlap");
+}
 
 void qk_norm_rope_op(const at::Tensor& qkv, const at::Tensor& pos, const at::Tensor& inv_freq, const at::Tensor& axis,
                      at::Tensor& q_out, at::Tensor& k_cache, at::Tensor& v_cache, int64_t heads, int64_t kv_heads,
@@ -171,9 +175,9 @@ void qk_norm_rope_op(const at::Tensor& qkv, const at::Tensor& pos, const at::Ten
   APPCORR_CHECK(head_dim == 64 || head_dim == 128, "qk_norm_rope: head_dim must be 64 or 128, got ", head_dim);
   APPCORR_CHECK(heads > 0 && kv_heads > 0, "qk_norm_rope: heads and kv_heads must be positive");
   check_rows_bf16(qkv, "qkv", (heads + 2 * kv_heads) * head_dim);
-  check_rows_bf16(q_out, "q_out", heads * head_dim);
-  check_rows_bf16(k_cache, "k_cache", kv_heads * head_dim);
-  check_rows_bf16(v_cache, "v_cache", kv_heads * head_dim);
+  check_written_rows(q_out, "q_out", heads * head_dim);
+  check_written_rows(k_cache, "k_cache", kv_heads * head_dim);
+  check_written_rows(v_cache, "v_cache", kv_heads * head_dim);
   const int64_t N = qkv.size(0);
   APPCORR_CHECK(N < (int64_t(1) << 31), "qk_norm_rope: too many tokens");
   APPCORR_CHECK(q_out.size(0) >= N, "qk_norm_rope: q_out has ", q_out.size(0), " rows for ", N, " tokens");

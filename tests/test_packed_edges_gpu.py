@@ -201,3 +201,22 @@ def test_single_values_of_any_stride():
     c.prefix_table = torch.stack([c.prefix_table] * 2, 1)[:, 0]
     c.run(kv_len=one(100))
     c.check()
+
+
+def test_rope_refuses_outputs_whose_rows_overlap():
+    N, H, K, D = 4, 2, 1, 64
+    z = lambda *s, dtype=torch.bfloat16: torch.zeros(*s, device=DEV, dtype=dtype)  # noqa: E731
+
+    def call(**kw):
+        a = dict(qkv=z(N, (H + 2 * K) * D), q=z(N, H * D), k=z(N, K * D), v=z(N, K * D)) | kw
+        _packed().qk_norm_rope(a["qkv"], z(1, N, dtype=torch.int32), z(D // 2, dtype=torch.float32), z(D // 2, dtype=torch.int32), a["q"],
+                               a["k"], a["v"], heads=H, kv_heads=K, head_dim=D)
+
+    for name, width in (("q", H * D), ("k", K * D), ("v", K * D)):
+        for row in (0, 8, width - 8):
+            with pytest.raises(RuntimeError, match="rows must not overlap"):
+                call(**{name: z(N * width).as_strided((N, width), (row, 1))})
+    call(qkv=z(1, (H + 2 * K) * D).expand(N, -1))  # read only: every token alike
+    pool = z(N, 2, K * D)
+    call(k=pool[:, 0], v=pool[:, 1])  # caches side by side in one pool
+    _done()
