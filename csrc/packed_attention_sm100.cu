@@ -422,7 +422,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int t0 = t * tt2, ntok = min(tt2, r.q - t0);
         const int vis1 = r.shared ? r.kv : min(max(r.past + t0 + ntok, 0), r.kv);
         const int vis0 = r.shared ? r.kv : min(max(r.past + t0 + min(ntok, p.TT), 0), r.kv);
-        const int nb = (vis1 + kBlk - 1) / kBlk, nb0 = (vis0 + kBlk - 1) / kBlk;
+        const int nb = vis1 / kBlk + (vis1 % kBlk != 0), nb0 = vis0 / kBlk + (vis0 % kBlk != 0);
         const bool owner = at >= w0;
         const int jb = cut_block(w0, at, cost, nb, ntok <= p.TT, r.fixed), je = cut_block(w1, at, cost, nb, ntok <= p.TT, r.fixed);
         const bool whole = jb == 0 && je == nb;
@@ -484,7 +484,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               row = __shfl_sync(0xffffffffu, pg, j & 31) * kBlk;
             } else {
               const int k0 = p.k_start[b];
-              row = k0 >= 0 && k0 < p.key_rows ? k0 + blk * kBlk : p.key_rows;
+              row = k0 >= 0 && blk <= (p.key_rows - k0) / kBlk ? k0 + blk * kBlk : p.key_rows;
             }
 #pragma unroll
             for (int kv = 0; kv < 2; ++kv) {

@@ -220,3 +220,26 @@ def test_rope_refuses_outputs_whose_rows_overlap():
     pool = z(N, 2, K * D)
     call(k=pool[:, 0], v=pool[:, 1])  # caches side by side in one pool
     _done()
+
+
+# ------------------------------------------------------------------------------------ key lengths near 2^31
+@pytest.mark.parametrize("paged,own", [(True, TOP), (True, TOP - 127), (False, TOP - 40)])
+def test_attention_key_lengths_near_the_largest(paged, own):
+    """Far more keys than there are rows: the missing ones are rows of zeros, as everywhere, and count. (A
+    sum of 2^31 terms in fp32, 2^24 of them per block at the most, is off by less than 2^-11.)"""
+    c = Case([1, 2], [200, 2], 4, 2, 64, seed=79, paged=paged)
+    if paged:
+        c.table = c.table[:, :2].contiguous()
+        rest = int(c.rows[0][199]) + 1  # the second page's other rows are keys here
+        c.k[rest:rest + 56], c.v[rest:rest + 56] = 0, 0
+    else:
+        c.k_start, c.k, c.v = _i([3, 0]), c.k[c.rows[0]].contiguous(), c.v[c.rows[0]].contiguous()
+        c.rows = [torch.arange(3, 200, device=DEV), torch.arange(2, device=DEV)]
+    c.run(kv_len=_i([own, 2]))
+    k, v = (x[c.rows[0]].double().view(-1, 2, 64) for x in (c.k, c.v))
+    for h in range(4):
+        x = k[:, h // 2] @ c.q[0, h * 64:(h + 1) * 64].double() / 8
+        total = x.exp().sum() + (own - x.numel())
+        o, size = x.exp() @ v[:, h // 2] / total, x.exp() @ v[:, h // 2].abs() / total
+        assert bool(((c.o[0, h * 64:(h + 1) * 64].double() - o).abs() <= 2.0 ** -8 * o.abs() + (2.0 ** -8 + 2.0 ** -11) * size).all())
+        assert abs(float(c.lse[0, h].double() - total.log())) <= 2.0 ** -11 + 2.0 ** -20 * 22
