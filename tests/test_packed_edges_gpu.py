@@ -243,3 +243,31 @@ def test_attention_key_lengths_near_the_largest(paged, own):
         o, size = x.exp() @ v[:, h // 2] / total, x.exp() @ v[:, h // 2].abs() / total
         assert bool(((c.o[0, h * 64:(h + 1) * 64].double() - o).abs() <= 2.0 ** -8 * o.abs() + (2.0 ** -8 + 2.0 ** -11) * size).all())
         assert abs(float(c.lse[0, h].double() - total.log())) <= 2.0 ** -11 + 2.0 ** -20 * 22
+
+
+# ------------------------------------------------------------------------------------ streams
+@pytest.mark.parametrize("prefix", [0, 1500])
+def test_calls_on_two_streams_keep_apart(prefix):
+    """Many calls in flight on two streams at once, every one into an output of its own that held NaN: the
+    same bits as a call by itself. Nothing is uploaded or read in between."""
+    P, calls = _packed(), 12
+    cases = [Case([1] * 9, [700 + 111 * i for i in range(9)], 28, 4, 128, prefix=prefix, seed=s) for s in (83, 89)]
+    want, args, outs = [], [], []
+    for c in cases:
+        c.run()
+        c.check()
+        want.append((c.o.clone(), c.lse.clone()))
+        args.append(dict(q_start=_i(c.start), kv_len=_i(c.own), heads=28, kv_heads=4, head_dim=128, table=c.table) |
+                    (dict(prefix_table=c.prefix_table, prefix_len=prefix) if prefix else {}))
+        outs.append([(torch.full_like(c.o, float("nan")), torch.full_like(c.lse, float("nan"))) for _ in range(calls)])
+    fn = P.shared_prefix_attention if prefix else P.packed_attention
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    for i in range(calls):
+        for c, a, out, s in zip(cases, args, outs, streams):
+            with torch.cuda.stream(s):
+                fn(c.q, c.k, c.v, out[i][0], lse=out[i][1], **a)
+    _done()
+    for (o, lse), out in zip(want, outs):
+        for got, got_lse in out:
+            assert torch.equal(got, o) and torch.equal(got_lse, lse)
