@@ -1024,9 +1024,9 @@ __global__ void __launch_bounds__(kJoinThreads, kCutBlocksPerSm) join_cut_tiles_
   if (tid < kMaxBlocks) {
     CutTile cut;
     cut.parts = -1;
-    const bool failed = error_raised(p.err);  // the parts are not there: no row is joined
+    const int failed = *p.err;  // the parts are not there: no row is joined
     if (tid < blocks) cut = p.cuts[tid];
-    if (failed) cut.parts = -1;
+    if (failed != 0) cut.parts = -1;
     s_cut[tid] = cut;
     rows = cut.parts >= 0 ? cut.ntok * p.G : 0;
 #pragma unroll
@@ -1069,10 +1069,10 @@ __global__ void __launch_bounds__(kJoinThreads) join_rows_kernel(PackedAttnParam
   let_later_kernels_start();
   const long cls = (long)p.N * p.H, orow = (long)blockIdx.x * (kJoinThreads / 32) + (threadIdx.x >> 5);
   if (orow >= cls) return;
-  const bool failed = error_raised(p.err);
-  const int own = p.row_parts[orow], pre = p.row_parts[cls + orow];
+  const int failed = *p.err, own = p.row_parts[orow], pre = p.row_parts[cls + orow];
+  const int from = p.q_start[0], to = p.q_start[p.B];
   const int tok = static_cast<int>(orow / p.H), head = static_cast<int>(orow - (long)tok * p.H);
-  if (failed || tok < p.q_start[0] || tok >= p.q_start[p.B]) return;  // no parts; no request's row
+  if ((failed != 0) | (tok < from) | (tok >= to)) return;  // no parts; no request's row (five reads at once)
   auto whole = [](int parts) { return (parts & 0xffffff) == kWholeRow; };
   const int n_own = whole(own) ? 1 : part_count(own), n_pre = whole(pre) ? 1 : part_count(pre);
   const int own_row = static_cast<unsigned>(own) >> 24, pre_row = static_cast<unsigned>(pre) >> 24;
