@@ -134,6 +134,18 @@ __device__ __forceinline__ Request load_request(const PackedAttnParams& p, int i
   if (b < 0) return make_request(p, p.q_start[0], p.q_start[p.B], p.shared_len, true);
   return make_request(p, p.q_start[b], p.q_start[b + 1], p.kv_len[b], false);
 }
+// the first entry from i on that has new tokens (a whole warp looks, 32 at a time: one after another they
+// took 0.2 us each, 3.3 ms for 16384 of them), or E; i lies behind the prefix's entry
+__device__ __forceinline__ int next_entry(const PackedAttnParams& p, int i, int E) {
+  const int lane = threadIdx.x & 31, b0 = p.shared_len > 0 ? 1 : 0;
+  for (; i < E; i += 32) {
+    const int b = i + lane - b0;
+    const bool some = i + lane < E && min(p.q_start[b + 1], p.N) > max(p.q_start[b], 0);
+    const unsigned found = __ballot_sync(0xffffffffu, some);
+    if (found) return i + __ffs(found) - 1;
+  }
+  return E;
+}
 // cost of the first k tiles of one head
 __device__ __forceinline__ long tiles_cost(const Request& r, int k) {
   long c = k * r.base + (long)r.slope * k * (k + 1) / 2;
@@ -522,11 +534,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           t = 0;
           if (++hv == p.Hv) {
             hv = 0;
-            do {
-              if (++e >= E) break;
-              r = load_request(p, e);
-            } while (r.nt == 0);
+            if (at >= w1) break;  // before looking further: what follows may be thousands of idle requests
+            e = next_entry(p, e + 1, E);
             if (e >= E) break;
+            r = load_request(p, e);
           }
         }
       }

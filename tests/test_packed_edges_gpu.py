@@ -271,3 +271,46 @@ def test_calls_on_two_streams_keep_apart(prefix):
     for (o, lse), out in zip(want, outs):
         for got, got_lse in out:
             assert torch.equal(got, o) and torch.equal(got_lse, lse)
+
+
+# ------------------------------------------------------------------------------------ idle requests
+def _slots(B, active, prefix):
+    q_len, own = [0] * B, [300] * B
+    for b, n, keys in active:
+        q_len[b], own[b] = n, keys
+    c = Case([n for n in q_len if n], [k for n, k in zip(q_len, own) if n], 4, 2, 64, prefix=prefix, seed=97)
+    at, start, table = [b for b, n in enumerate(q_len) if n], [0], torch.full((B, c.table.shape[1]), 1 << 30, dtype=torch.int32)
+    for n in q_len:
+        start.append(start[-1] + n)
+    table[at] = c.table.cpu()
+    return c, dict(q_start=_i(start), kv_len=_i(own), table=table.to(DEV))
+
+
+@pytest.mark.parametrize("prefix", [0, 300])
+@pytest.mark.parametrize("B,active", [(40, (0, 39)), (700, (0, 31, 32, 33, 64, 699)), (700, (650,)), (3000, (1, 2998)), (33, (32,)), (34, (1, 33))])
+def test_attention_between_idle_requests(B, active, prefix):
+    """Requests without new tokens (whose tables hold no page) before, between and behind the active ones."""
+    c, kw = _slots(B, [(b, 1 + 70 * (i & 1), 600 + 100 * i) for i, b in enumerate(active)], prefix)
+    c.run(**kw)
+    c.check()
+
+
+@pytest.mark.parametrize("prefix", [0, 300])
+def test_idle_requests_cost_little(prefix):
+    """A few requests ahead of thousands of idle ones take no multiple of what as many, spread out, take."""
+    times = []
+    for active in (range(64), range(0, 16384, 256)):
+        c, kw = _slots(16384, [(b, 1, 600) for b in active], prefix)
+        c.run(**kw)
+        ev = [torch.cuda.Event(enable_timing=True) for _ in range(6)]
+        for e in ev:  # the outputs of the first call stay in c.o
+            e.record()
+            if prefix:
+                _packed().shared_prefix_attention(c.q, c.k, c.v, c.o, prefix_table=c.prefix_table, prefix_len=prefix, heads=4, kv_heads=2, head_dim=64, **kw)
+            else:
+                _packed().packed_attention(c.q, c.k, c.v, c.o, heads=4, kv_heads=2, head_dim=64, **kw)
+        torch.cuda.synchronize()
+        times.append(min(a.elapsed_time(b) for a, b in zip(ev, ev[1:])))
+        c.run(**kw)
+        c.check()
+    assert times[0] < 4 * times[1], times
