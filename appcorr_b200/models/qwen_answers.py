@@ -71,6 +71,7 @@ class PackedAnswers:
         if engine.fp8:
             self.t["a8"] = torch.empty(max_step, max(D, engine.nffn), device=dev, dtype=torch.float8_e4m3fn)
             self.t["a8s"] = torch.empty(max_step, device=dev, dtype=torch.float32)
+        self.zero = torch.zeros(1, device=dev, dtype=torch.int64)
         self.reset()
 
     def reset(self) -> None:
@@ -79,7 +80,7 @@ class PackedAnswers:
         self.held = z(self.max_requests)          # own tokens of each request so far
         self.free_at = z(2)                       # next free page, blocks that went without one
         self.t["last"].zero_()                    # normalised last row of each request
-        self.short = torch.zeros((), device=self.engine.device, dtype=torch.int64)  # tokens that ids did not hold
+        self.asked = torch.zeros_like(self.zero)  # tokens that q_len has named
 
     def step(self, ids: torch.Tensor, q_len: torch.Tensor) -> torch.Tensor:
         """ids int32 (N values): the new tokens, request by request; q_len int32 [B] how many each brings.
@@ -96,12 +97,11 @@ class PackedAnswers:
         N, B = ids.numel(), q_len.numel()
         if N > self.max_step or B > self.max_requests:
             raise ValueError(f"{N} tokens of {B} requests: this batch holds {self.max_step} of {self.max_requests}")
-        ends = q_len.clamp(min=0).cumsum(0)
-        held = torch.nn.functional.pad(ends.clamp(max=N), (1, 0))  # of each request, the tokens that are there
         if B:
-            self.short += ends[-1] - held[-1]
-        if N:
-            self._layers(ids, held.diff().to(torch.int32))
+            ends = q_len.clamp(min=0).cumsum(0)
+            self.asked += ends[-1]
+        if B and N:  # of each request, the tokens that are there
+            self._layers(ids, torch.diff(ends.clamp_(max=N), prepend=self.zero).to(torch.int32))
         logits = t["logits"][:B]
         if B:
             K.gemm(t["last"][:B], eng.lm_head, logits, epi=K.EPI_F32)
@@ -144,7 +144,7 @@ class PackedAnswers:
         self.free_at = free_at
         last = t["last"][:B]
         ends = torch.empty_like(last)
-        K.rmsnorm(x, eng.norm, c.rms_eps, ends, rows=(q_start[1:] - 1).clamp(0, N - 1))
+        K.rmsnorm(x, eng.norm, c.rms_eps, ends, rows=q_start[1:].clamp(min=1).sub_(1))
         torch.where(q_len[:, None] > 0, ends, last, out=last)
 
     @property
@@ -155,7 +155,7 @@ class PackedAnswers:
     @property
     def tokens_missing(self) -> int:
         """Tokens named by q_len that ids did not hold so far (synchronises)."""
-        return int(self.short)
+        return int(self.asked - self.held.sum())
 
     def generate(self, questions: List[torch.Tensor], n: int) -> torch.Tensor:
         """Greedy answers of n tokens to the questions (int32 token ids each) -> int32 [B, n]. Raises where
