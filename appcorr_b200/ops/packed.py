@@ -13,7 +13,8 @@ All tensors are CUDA tensors; outputs are given by the caller, as in ops/kernels
 launches on the current stream without synchronising. Cache pages hold 128 rows of [kv_heads *
 head_dim] bf16. Shapes, types and devices are checked in the C++ bindings; values on the device
 (lengths, pages, rows) are not read by the host: a page or row outside its pool is never written, and
-as a key it reads as a row of zeros.
+as a key it reads as a row of zeros. After an error that a kernel has recorded (ops/native.check_errors)
+rows of the attention may stay as they were.
 """
 from __future__ import annotations
 

@@ -35,13 +35,14 @@
 // their V rows are zeroed in shared memory, since 0 * NaN would reach the accumulators.
 // All waits are bounded; a wait that runs out sets the error word, every role leaves and no row is joined.
 //
-// What bounds it. Long prompts (four of 3010 to 5001 tokens, 28 heads of 128 over 4, 487 GFLOP): 480 to 510
-// us, about 1 PFLOP/s. A key block of a half is 3700 clocks from one S to the next: 2000 of softmax
+// What bounds it. Long prompts (four of 3010 to 5001 tokens, 28 heads of 128 over 4, 487 GFLOP): 483 to 498
+// us at 1965 MHz (a few calls, 0.98 to 1.01 PFLOP/s), 544 us (0.90) at the 1720 to 1740 MHz that the power
+// limit leaves after a second of them. A key block of a half is 3700 clocks from one S to the next: 2000 of softmax
 // (exponentials 1280, at the special-function unit's rate; maxima 390; TMEM reads and writes 310), 1024
 // of products, the rest hand-offs; the tensor core is busy a little over half of the time. Tried and not
 // kept: a quarter or half of the exponentials on the fp32 pipe (equal / 10 % slower), 16 softmax warps
 // with a row over four lanes (equal on prompts, 1 us slower on small calls). Answers (96 of 60 to 6000
-// keys, 237 MB): 60 to 62 us, 3.9 TB/s; each SM's stretches hold 1 to 10 tiles, and a tile's turnaround (3.6 us:
+// keys, 237 MB): 59 to 64 us, 3.7 to 4.0 TB/s; each SM's stretches hold 1 to 10 tiles, and a tile's turnaround (3.6 us:
 // last product, output, next tile's first scores) is only partly covered by the loads ahead of it. Small
 // calls (10 us): 2 us of work line, 1.5 us of loads, 1.3 us for the first softmax, 1 us of output, and the
 // joining kernel.

@@ -11,7 +11,9 @@
 // formed in one fp32 product would be off by 1e-3 rad at position 30000.
 //
 // Bound: HBM, every projected value read once and written once (20011 tokens of 48 heads x 64: 246 MB in
-// 46 us = 5.3 TB/s, 0.83 of a plain copy; 1424 tokens of 36 x 128: 26 MB in 5.5 us; 61 of them: 2.9 us).
+// 46.7 us = 5.3 TB/s, 0.82 of a plain copy). At 1 to 2 waves of blocks it is the latency of a load, sines,
+// store chain: 1424 tokens of 36 heads x 128, 26 MB, take 7.5 us without norms and 8.3 with them where the
+// inputs come from HBM, 5.1 and 6.2 where L2 still holds them; 61 of them with norms 2.7 us.
 // A lane holds 8 values of a head's first half and the 8 they are paired with, so both loads and
 // stores are 16 bytes and the rotation needs no exchange; a head is D / 16 lanes (the norm is 3 or
 // 2 shuffles) and a warp walks its token's heads 32 / (D / 16) at a time with the next ones' loads
@@ -217,8 +219,9 @@ void qk_norm_rope_op(const at::Tensor& qkv, const at::Tensor& pos, const at::Ten
                static_cast<int>(heads), static_cast<int>(kv_heads)};
   auto st = at::cuda::getCurrentCUDAStream();
   // Warps per token: fewer repeat the sines less, more shorten the chain of a single token. Measured in us
-  // at 1 / 2 / 4 / 8 with 36 heads x 128: 61 tokens 5.4 / 4.1 / 3.3 / 2.8, 600: 5.6 / 4.8 / 4.4 / 5.0,
-  // 1424: 7.4 / 6.4 / 6.5 / 8.3, 3000: 9.9 / 10.8 / 11.6 / 14.7, 20011: 66 / 69 / 78 / 103.
+  // at 1 / 2 / 4 / 8 with 36 heads x 128 and norms, inputs from HBM (from L2): 61 tokens 5.9 / 4.2 / 3.5 / 2.8
+  // (5.1 / 3.9 / 3.1 / 2.6), 600: 8.7 / 6.6 / 5.5 / 6.3 (5.4 / 4.6 / 4.2 / 4.7), 1424: 10.2 / 8.3 / 9.3 / 10.7
+  // (7.2 / 6.2 / 6.3 / 8.1), 3000: 13.0 / 13.9 / 15.3 / 18.4, 20011: 67 / 70 / 79 / 104.
   const int wpt = N >= 2048 ? 1 : (N >= 1024 ? 2 : (N >= 512 ? 4 : 8));
   auto go = [&](auto kern) {
     const long per = kRopeThreads / 32 / wpt;

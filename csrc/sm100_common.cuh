@@ -2,9 +2,10 @@
 //
 // Thin inline-PTX wrappers for the Blackwell primitives the kernels are built from:
 // mbarriers, TMA tiled loads (cp.async.bulk.tensor), tcgen05 TMEM allocation, tcgen05.mma,
-// tcgen05.commit and tcgen05.ld. Every wait on an mbarrier is bounded by a wall-clock budget read
-// from %globaltimer; on expiry the waiter records an error code in a device word that the host
-// checks, and returns false so the calling role can leave its loop instead of spinning forever.
+// tcgen05.commit and tcgen05.ld. Every wait on an mbarrier is bounded, by a wall-clock budget read
+// from %globaltimer (mbar_wait) or by a count of polls (the packed attention's own); on expiry the
+// waiter records an error code in a device word that the host checks, and returns false so the
+// calling role can leave its loop instead of spinning forever.
 #pragma once
 #include <cstdint>
 #include <cuda.h>
